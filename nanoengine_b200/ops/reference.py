@@ -8,7 +8,7 @@ experts/generic.py:237-273, attention/base.py:451-525 SDPA reference, layers/sam
 from __future__ import annotations
 
 import math
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -340,8 +340,105 @@ def mla_kv_store(cache: torch.Tensor, slot_mapping: torch.Tensor, ckv: torch.Ten
         flat[slots] = row.to(cache.dtype)
 
 
+# ---- 4-bit rows ----------------------------------------------------------------------------------
+# A key / value cache held in 4 bits: uint8 [blocks, kv heads, block_size * (D / 2 + D / 32)].  A page holds, for every kv head, the codes of its
+# tokens (D / 2 bytes each) and behind them their scales (a byte for each group of 32 neighbouring dims).  Scale byte 8 e + m stands for
+# (8 + m) 2^(e - 19): 2^-16 to 1.875 * 2^15, no zero, no infinity, no NaN.  Code c of 0 .. 15 stands for (c - 8) scale.  A row's codes are 32-bit
+# words of 8 dims, the dims of even place in the low half, the others in the high half, lowest dim in the lowest bits: a kernel that shifts and masks
+# a word gets two neighbouring dims side by side.  Products of a code and a scale have at most 7 significant bits: exact in bf16.
+KV4_GROUP = 32
+KV4_ORDER = [0, 2, 4, 6, 1, 3, 5, 7]          # dim of a word's nibble p
+
+
+def kv4_page_bytes(dim: int, block_size: int) -> int:
+    """Bytes of one kv head's rows in one page: the last size of a 4-bit cache."""
+    if dim % KV4_GROUP or dim < KV4_GROUP:
+        raise ValueError("4-bit rows need a head size that is a multiple of 32")
+    return block_size * (dim // 2 + dim // KV4_GROUP)
+
+
+def kv4_block_size(cache: torch.Tensor, dim: int) -> int:
+    """Tokens per page of a 4-bit cache of heads of `dim`."""
+    row = kv4_page_bytes(dim, 1)
+    if cache.dtype != torch.uint8 or cache.dim() != 3 or cache.shape[2] % row or cache.shape[2] < row:
+        raise ValueError(f"a 4-bit cache of heads of {dim} is uint8 [blocks, kv heads, block_size * {row}], not {cache.dtype} {list(cache.shape)}")
+    return cache.shape[2] // row
+
+
+def kv4_quant(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """x [..., D] -> (codes uint8 [..., D / 2], scale bytes uint8 [..., D / 32]).  The scale is the nearest of the 256 (on a logarithmic grid of four
+    significant bits, ties to even) to a seventh of the group's largest magnitude, a code the nearest multiple from -7 to 7.  Infinities and values
+    past 7 times the largest scale become the largest that the format holds, a NaN becomes 0.  Decided in 64 bits, where every quotient that lies
+    on a border of bf16 rows is exact: equal rows give equal bytes whatever order their norm was summed in."""
+    if x.shape[-1] % KV4_GROUP:
+        raise ValueError("4-bit rows need a head size that is a multiple of 32")
+    most = 7 * 1.875 * 2.0 ** 15
+    g = torch.nan_to_num(x.double(), nan=0.0, posinf=most, neginf=-most).clamp(-most, most).reshape(*x.shape[:-1], -1, KV4_GROUP)
+    m, e = torch.frexp(g.abs().amax(-1) / 7)              # m in [1/2, 1)
+    n = torch.round(m * 16).long()                        # 8 .. 16, or 0
+    b = 8 * (e.long() + 15) + n - 8                       # n = 16 carries into the next power of two by itself
+    b = torch.where(n == 0, torch.zeros_like(b), b.clamp(0, 255))
+    s = torch.ldexp((8 + (b & 7)).double(), (b >> 3) - 19)
+    c = torch.round(g / s[..., None]).clamp(-7, 7).long() + 8
+    c = c.reshape(*x.shape[:-1], -1, 8)[..., KV4_ORDER]
+    return (c[..., 0::2] + 16 * c[..., 1::2]).to(torch.uint8).reshape(*x.shape[:-1], -1), b.to(torch.uint8)
+
+
+def kv4_values(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """The rows [..., D] (fp32) that codes [..., D / 2] and scale bytes [..., D / 32] stand for."""
+    n = torch.stack([codes & 15, codes >> 4], -1).reshape(*codes.shape[:-1], -1, 8)
+    n = n[..., [KV4_ORDER.index(i) for i in range(8)]].reshape(*codes.shape[:-1], -1).float() - 8
+    b = scales.int()
+    return n * torch.ldexp((8 + (b & 7)).float(), (b >> 3) - 19).repeat_interleave(KV4_GROUP, -1)
+
+
+def _kv4_parts(cache: torch.Tensor, dim: int):
+    """Views (codes [blocks, heads, block_size, D / 2], scales [blocks, heads, block_size, D / 32]) of a 4-bit cache."""
+    bs = kv4_block_size(cache, dim)
+    split = bs * dim // 2
+    return cache[..., :split].unflatten(-1, (bs, dim // 2)), cache[..., split:].unflatten(-1, (bs, dim // KV4_GROUP))
+
+
+def _kv4_store(cache: torch.Tensor, slot_mapping: torch.Tensor, x: torch.Tensor) -> None:
+    codes, scales = _kv4_parts(cache, x.shape[-1])
+    bs = codes.shape[2]
+    keep = (slot_mapping >= 0) & (slot_mapping < cache.shape[0] * bs)
+    slots = slot_mapping[keep].long()
+    c, s = kv4_quant(x[keep])
+    codes[slots // bs, :, slots % bs] = c
+    scales[slots // bs, :, slots % bs] = s
+
+
+def _kv4_context_rows(cache: torch.Tensor, block_table: torch.Tensor, n: int, dim: int) -> torch.Tensor:
+    """Rows [n, heads, D] of one sequence's context; those of a page id outside the cache are zeros."""
+    codes, scales = _kv4_parts(cache, dim)
+    bs = codes.shape[2]
+    pages = block_table[: -(-n // bs)].long()
+    there = (pages >= 0) & (pages < cache.shape[0])
+    pages = torch.where(there, pages, torch.zeros_like(pages))
+    rows = kv4_values(codes[pages], scales[pages]) * there.view(-1, 1, 1, 1)
+    return rows.transpose(1, 2).flatten(0, 1)[:n]
+
+
+def gqa_kv_gather(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, dim: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows `slots` of 4-bit caches as values: (k, v), bf16 [T, kv heads, dim] each, every value exact.  A slot outside the cache (-1) gives zeros."""
+    out = []
+    for cache in (k_cache, v_cache):
+        codes, scales = _kv4_parts(cache, dim)
+        bs = codes.shape[2]
+        there = (slots >= 0) & (slots < cache.shape[0] * bs)
+        s = torch.where(there, slots, torch.zeros_like(slots)).long()
+        rows = kv4_values(codes[s // bs, :, s % bs], scales[s // bs, :, s % bs])
+        out.append((rows * there.view(-1, 1, 1)).to(torch.bfloat16))
+    return out[0], out[1]
+
+
 def gqa_kv_store(k_cache, v_cache, slot_mapping, k, v) -> None:
-    """k_cache/v_cache [blocks, block_size, kv_heads, head_dim]."""
+    """k_cache/v_cache [blocks, block_size, kv_heads, head_dim], or 4-bit pages uint8 [blocks, kv_heads, kv4_page_bytes] (there slot -1 writes nothing)."""
+    if k_cache.dtype == torch.uint8:
+        _kv4_store(k_cache, slot_mapping, k)
+        _kv4_store(v_cache, slot_mapping, v)
+        return
     k_cache.view(-1, *k_cache.shape[2:])[slot_mapping.long()] = k.to(k_cache.dtype)
     v_cache.view(-1, *v_cache.shape[2:])[slot_mapping.long()] = v.to(v_cache.dtype)
 
@@ -383,14 +480,58 @@ def conv_rows(proj: torch.Tensor, w: torch.Tensor, q_width: int, k_cache, v_cach
     return y[:, :q_width].contiguous()
 
 
+def angle_axes(half: int, sections: Sequence[int], interleaved: bool) -> torch.Tensor:
+    """Which position axis each of the `half` rotary angles of a head follows, int64 [half].  By sections: the first sections[0] angles the first axis,
+    the next sections[1] the second, and so on.  `interleaved`: axis a >= 1 has the angles a, a + A, a + 2 A, ... (A axes), sections[a] of them
+    or as many as the head has, the first axis all others."""
+    sections = [int(n) for n in sections]
+    if sum(sections) != half or min(sections) < 0 or not 1 <= len(sections) <= 4:
+        raise ValueError(f"sections {sections}: one to four axes whose angles add up to half a head, {half}")
+    A = len(sections)
+    if not interleaved:
+        return torch.repeat_interleave(torch.arange(A), torch.tensor(sections))
+    i = torch.arange(half)
+    a = i % A
+    return torch.where((a > 0) & (i < A * torch.tensor(sections)[a]), a, torch.zeros_like(a))
+
+
+def rope_axes_rows(positions: torch.Tensor, rope_cache: torch.Tensor, sections: Sequence[int], interleaved: bool = False) -> torch.Tensor:
+    """Rows [T, D] (cos | sin) of the rotation of tokens with a position per axis, positions [A, T]."""
+    half = rope_cache.shape[1] // 2
+    if positions.dim() != 2 or positions.shape[0] != len(sections):
+        raise ValueError(f"positions {list(positions.shape)}: one row per axis of sections {list(sections)}")
+    place = positions.long().t()[:, angle_axes(half, sections, interleaved).to(positions.device)]
+    i = torch.arange(half, device=positions.device)
+    return torch.cat([rope_cache[place, i], rope_cache[place, i + half]], -1)
+
+
 def gqa_qkv_prepare(qkv: torch.Tensor, hq: int, hkv: int, hd: int, q_norm_w, k_norm_w, eps: float, unit_offset: bool, positions,
-                    rope_cache: torch.Tensor, k_cache, v_cache, slot_mapping) -> torch.Tensor:
+                    rope_cache: torch.Tensor, k_cache, v_cache, slot_mapping, sections: Optional[Sequence[int]] = None, interleaved: bool = False) -> torch.Tensor:
     """The GQA front end after the qkv projection: split [T, (hq + 2 hkv) * hd] into heads, per-head RMSNorm of q and k (when
     the weights are given), rotary embedding of both over the whole head (pairs (i, i + hd/2)), K and V rows stored into their
-    paged cache slots.  Returns q [T, hq, hd] (reference models/qwen3_moe/qwen3_moe.py:58-146, triton/generic/kv_store.py:7)."""
+    paged cache slots.  Returns q [T, hq, hd] (reference models/qwen3_moe/qwen3_moe.py:58-146, triton/generic/kv_store.py:7).
+    `sections`: positions [A, T] hold one position per axis (time, height, width of image and video tokens) and every angle follows the axis that
+    `angle_axes` gives it.  uint8 caches hold 4-bit rows (`kv4_quant`).  In both forms a row is rounded once, behind the rotation, and the key that
+    is cut to 4 bits is computed in 64 bits."""
     T = qkv.shape[0]
     q, k, v = qkv.split([hq * hd, hkv * hd, hkv * hd], -1)
     q, k, v = q.reshape(T, hq, hd), k.reshape(T, hkv, hd), v.reshape(T, hkv, hd)
+    if sections is not None or k_cache.dtype == torch.uint8:
+        if rope_cache.shape[1] != hd:
+            raise ValueError("the rotary table covers another head size")
+        turn = rope_cache[positions.long()] if sections is None else rope_axes_rows(positions, rope_cache, sections, interleaved)
+        wide = torch.float64 if k_cache.dtype == torch.uint8 else torch.float32
+
+        def row(x, w, t):
+            x = x.to(t)
+            if w is not None:
+                x = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps) * (w.to(t) + (1.0 if unit_offset else 0.0))
+            (a, b), (cos, sin) = x.chunk(2, -1), turn.to(t)[:, None].chunk(2, -1)
+            return torch.cat([a * cos - b * sin, b * cos + a * sin], -1)
+
+        keep = slot_mapping >= 0
+        gqa_kv_store(k_cache, v_cache, slot_mapping[keep], row(k, k_norm_w, wide)[keep], v[keep])
+        return row(q, q_norm_w, torch.float32).to(qkv.dtype)
     if q_norm_w is not None:
         q = rmsnorm(q.reshape(-1, hd), q_norm_w, eps, False, unit_offset).view(T, hq, hd)
     if k_norm_w is not None:
@@ -400,6 +541,82 @@ def gqa_qkv_prepare(qkv: torch.Tensor, hq: int, hkv: int, hd: int, q_norm_w, k_n
     keep = slot_mapping >= 0
     gqa_kv_store(k_cache, v_cache, slot_mapping[keep], k[keep], v[keep])
     return q
+
+
+# ---- tables of a step --------------------------------------------------------------------------------------
+class StepTables(NamedTuple):
+    """What the kernels of one paged step read about its sequences (`step_tables`)."""
+    cu_seqlens_q: torch.Tensor         # int32 [rows + 1]
+    context_lens: torch.Tensor         # int32 [rows]
+    positions: torch.Tensor            # int64 [tokens]
+    slot_mapping: torch.Tensor         # int64 [tokens]
+    block_tables: torch.Tensor         # int32 [rows, max_blocks]
+    last_token_indices: torch.Tensor   # int32 [rows]
+
+
+def _step_sizes(num_seqs: int, block_size: int, num_tokens: int, max_blocks: int, rows: Optional[int], pad_len: int, scratch_block: int) -> int:
+    rows = num_seqs if rows is None else int(rows)
+    if rows < num_seqs or block_size < 1 or num_tokens < 0 or max_blocks < 1 or pad_len < 1:
+        raise ValueError("step_tables: rows at least the sequences, sizes of at least one")
+    if rows > num_seqs and not 0 <= scratch_block < 2 ** 31:
+        raise ValueError("step_tables: padding rows need a scratch block")
+    if rows > num_seqs and pad_len > max_blocks * block_size:
+        raise ValueError("step_tables: padding rows are longer than the tables")
+    return rows
+
+
+def step_tables(q_lens: torch.Tensor, seq_lens: torch.Tensor, block_ids: torch.Tensor, block_offsets: torch.Tensor, block_size: int, num_tokens: int,
+                max_blocks: int, rows: Optional[int] = None, pad_len: int = 1, scratch_block: int = -1, out: Optional[StepTables] = None) -> StepTables:
+    """The tables of a paged step from its sequences' lengths: sequence i brings q_lens[i] new tokens to a context of seq_lens[i] (with them) and
+    owns the pages block_ids[block_offsets[i] : block_offsets[i + 1]].  Token j of it stands at position seq_lens[i] - q_lens[i] + j, in slot
+    page * block_size + position % block_size; a position before the first or behind the sequence's pages, or a negative page, gives slot -1 (its row is
+    not stored).  `rows` beyond the sequences are padding: `pad_len` tokens of a one-sequence context on `scratch_block`.  Tokens behind the last
+    row's have position 0 and slot -1, table entries behind a sequence's pages are 0.  All lengths live on the device; `num_tokens` and `max_blocks`
+    are the sizes of the tables, what does not fit is cut off.  `out`: tables of at least these sizes, written in place; what lies behind stays."""
+    B = q_lens.numel()
+    rows = _step_sizes(B, block_size, num_tokens, max_blocks, rows, pad_len, scratch_block)
+    if seq_lens.numel() != B or block_offsets.numel() != B + 1:
+        raise ValueError("step_tables: one length per sequence and one offset more")
+    dev, more = q_lens.device, rows - B
+    ids = torch.cat([block_ids.long(), torch.zeros(1, dtype=torch.long, device=dev)])
+    n_ids = block_ids.numel()
+    pad = torch.full((more,), pad_len, dtype=torch.long, device=dev)
+    q, n = torch.cat([q_lens.long().clamp(min=0), pad]), torch.cat([seq_lens.long(), pad])
+    cu = torch.cat([torch.zeros(1, dtype=torch.long, device=dev), q.cumsum(0)])
+    lo, hi = block_offsets[:-1].long().clamp(0, n_ids), block_offsets[1:].long().clamp(0, n_ids)
+    col = torch.arange(max_blocks, device=dev)
+    has = col < (hi - lo)[:, None]
+    table = torch.where(has, ids[torch.where(has, lo[:, None] + col, n_ids)], 0)
+    table = torch.cat([table, torch.full((more, max_blocks), scratch_block, dtype=torch.long, device=dev)])
+    own_pages = torch.cat([(hi - lo).clamp(min=0), torch.full((more,), max_blocks, dtype=torch.long, device=dev)])
+    t = torch.arange(num_tokens, device=dev)
+    seq = (torch.searchsorted(cu, t, right=True) - 1).clamp(max=max(rows - 1, 0))
+    if rows:
+        place = n[seq] - q[seq] + t - cu[seq]
+        live = (t < cu[-1]) & (place >= 0)
+        place = torch.where(live, place, 0)
+        at = place // block_size
+        flat = torch.where(at < own_pages[seq], at + torch.cat([lo, torch.full((more,), n_ids, dtype=torch.long, device=dev)])[seq], n_ids)
+        page = torch.where(seq < B, ids[flat.clamp(max=n_ids)], scratch_block)
+        slot = torch.where(live & (at < own_pages[seq]) & (page >= 0), page * block_size + place % block_size, -1)
+    else:
+        place, slot = torch.zeros_like(t), torch.full_like(t, -1)
+    made = StepTables(cu.int(), n.int(), place, slot, table.int(), (cu[1:] - 1).int())
+    if out is None:
+        return made
+    sizes = [(rows + 1,), (rows,), (num_tokens,), (num_tokens,), (rows, max_blocks), (rows,)]
+    _check_step_out(out, sizes)
+    views = StepTables(*(o[tuple(slice(k) for k in size)] for o, size in zip(out, sizes)))
+    for v, m in zip(views, made):
+        v.copy_(m)
+    return views
+
+
+def _check_step_out(out, sizes) -> None:
+    for name, o, size in zip(StepTables._fields, out, sizes):
+        want = torch.int64 if name in ("positions", "slot_mapping") else torch.int32
+        if o.dtype != want or o.dim() != len(size) or any(have < need for have, need in zip(o.shape, size)) or (o.numel() and o.stride(-1) != 1):
+            raise ValueError(f"step_tables: out.{name} must be {want} of at least {list(size)} with unit inner stride")
 
 
 # ---- pooled rows --------------------------------------------------------------------------------------------
@@ -505,8 +722,12 @@ def mla_attention_paged(q: torch.Tensor, cache: torch.Tensor, block_tables: torc
 
 def gqa_attention_paged(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale, window: int = 0) -> torch.Tensor:
     """q [T, Hq, D]; caches [blocks, block_size, Hkv, D]; causal; returns [T, Hq, D].  `window` > 0: a query at position p sees
-    key positions (p - window, p] only (sliding-window layers, reference layers/backends/attention/base.py:527-707)."""
+    key positions (p - window, p] only (sliding-window layers, reference layers/backends/attention/base.py:527-707).
+    uint8 caches hold 4-bit rows, [blocks, Hkv, kv4_page_bytes]: there a page id outside the cache reads as rows of zeros, a context is cut off where its
+    block table ends, and a query that sees no key gives zeros."""
     T, Hq, D = q.shape
+    if k_cache.dtype == torch.uint8:
+        return _gqa_attention_kv4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale, window)
     Hkv = k_cache.shape[2]
     out = torch.zeros(T, Hq, D, dtype=torch.float32, device=q.device)
     B = cu_seqlens_q.numel() - 1
@@ -524,6 +745,38 @@ def gqa_attention_paged(q, k_cache, v_cache, block_tables, cu_seqlens_q, context
         if window > 0:
             s = s.masked_fill(keys <= pos - window, float("-inf"))
         out[lo:hi] = torch.einsum("thn,nhd->thd", torch.softmax(s, -1), v)
+    return out.to(q.dtype)
+
+
+def check_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor) -> Tuple[int, int]:
+    """(kv heads, block size) of 4-bit caches that fit the queries [T, Hq, D]."""
+    if v_cache.dtype != torch.uint8 or v_cache.shape != k_cache.shape:
+        raise ValueError("4-bit keys and values come in caches of one shape")
+    bs, hkv = kv4_block_size(k_cache, q.shape[2]), k_cache.shape[1]
+    if hkv < 1 or q.shape[1] % hkv or q.shape[1] < hkv:
+        raise ValueError(f"{q.shape[1]} query heads over {hkv} kv heads")
+    return hkv, bs
+
+
+def _gqa_attention_kv4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale, window: int) -> torch.Tensor:
+    T, Hq, D = q.shape
+    Hkv, bs = check_kv4(q, k_cache, v_cache)
+    out = torch.zeros(T, Hq, D, dtype=torch.float32, device=q.device)
+    for i in range(cu_seqlens_q.numel() - 1):
+        lo, hi = max(0, int(cu_seqlens_q[i])), min(T, int(cu_seqlens_q[i + 1]))
+        n, ql = min(int(context_lens[i]), block_tables.shape[1] * bs), int(cu_seqlens_q[i + 1]) - int(cu_seqlens_q[i])
+        if hi <= lo or n <= 0:
+            continue
+        k, v = (_kv4_context_rows(c, block_tables[i], n, D) for c in (k_cache, v_cache))
+        keys = torch.arange(n, device=q.device)
+        pos = torch.arange(n - ql, n - ql + hi - lo, device=q.device)[:, None]
+        seen = keys <= pos
+        if window > 0:
+            seen = seen & (keys > pos - window)
+        s = torch.einsum("tgrd,ngd->tgrn", q[lo:hi].float().unflatten(1, (Hkv, -1)), k) * scale
+        s = s.masked_fill(~seen[:, None, None], float("-inf"))
+        p = torch.where(seen.any(-1)[:, None, None, None], torch.softmax(s, -1), torch.zeros_like(s))
+        out[lo:hi] = torch.einsum("tgrn,ngd->tgrd", p, v).flatten(1, 2)
     return out.to(q.dtype)
 
 

@@ -632,8 +632,10 @@ def mla_kv_store(cache: torch.Tensor, slot_mapping: torch.Tensor, ckv: torch.Ten
 
 
 def gqa_kv_store(k_cache, v_cache, slot_mapping, k, v):
-    """k, v [T, Hkv, D] (row stride free) -> rows `slot_mapping` of the paged caches [blocks, block_size, Hkv, D]."""
+    """k, v [T, Hkv, D] (row stride free) -> rows `slot_mapping` of the paged caches [blocks, block_size, Hkv, D], or of 4-bit pages (uint8)."""
     T = k.shape[0]
+    if k_cache.dtype == torch.uint8:
+        return _kv4_store(k_cache, v_cache, slot_mapping, k, v)
     row = k.shape[1] * k.shape[2]
     ok = (k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16 and k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16
           and k_cache.is_contiguous() and v_cache.is_contiguous() and row % 8 == 0)
@@ -684,10 +686,14 @@ def _i64c(t):
     return t if (t.dtype == torch.int64 and t.is_contiguous()) else t.long().contiguous()
 
 
-def gqa_qkv_prepare(qkv, hq, hkv, hd, q_norm_w, k_norm_w, eps, unit_offset, positions, rope_cache, k_cache, v_cache, slot_mapping):
+def gqa_qkv_prepare(qkv, hq, hkv, hd, q_norm_w, k_norm_w, eps, unit_offset, positions, rope_cache, k_cache, v_cache, slot_mapping, sections=None,
+                    interleaved=False):
     """One kernel for head split, q / k RMSNorm, rotary embedding and the paged K / V store (head dim 128 or 256 with the whole
-    head rotated, bf16 caches); other shapes run the same steps as separate kernels."""
+    head rotated, bf16 caches); other shapes run the same steps as separate kernels.  Positions on several axes and 4-bit caches: one
+    kernel for head dims 32, 64, 128 and 256."""
     T = qkv.shape[0]
+    if sections is not None or k_cache.dtype == torch.uint8:
+        return _gqa_rows(qkv, hq, hkv, hd, q_norm_w, k_norm_w, eps, unit_offset, positions, rope_cache, k_cache, v_cache, slot_mapping, sections, interleaved)
     fused = (hd in (128, 256) and rope_cache.shape[1] == hd and qkv.dtype == torch.bfloat16 and qkv.stride(1) == 1 and qkv.stride(0) % 2 == 0
              and k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16 and k_cache.is_contiguous() and v_cache.is_contiguous()
              and rope_cache.dtype == torch.float32 and rope_cache.is_contiguous())
@@ -709,6 +715,176 @@ def gqa_qkv_prepare(qkv, hq, hkv, hd, q_norm_w, k_norm_w, eps, unit_offset, posi
                                  _c.c_float(1.0 if unit_offset else 0.0), _p(_i64c(positions)), _p(rope_cache), _p(q), _p(k_cache), _p(v_cache),
                                  _p(_i64c(slot_mapping)), _c.c_int(T), _st()), "ne_gqa_qkv_prepare")
     return q
+
+
+# ---- 4-bit rows, positions on several axes, tables of a step ---------------------------------------
+kv4_page_bytes, kv4_block_size = ref.kv4_page_bytes, ref.kv4_block_size
+StepTables = ref.StepTables
+KV4_DIMS = (32, 64, 128, 256)           # head sizes the row kernels are built for
+_FNS = {}
+
+
+def _fn(name: str, spec: str):
+    """A C entry with declared arguments (p pointer, i int, l 64-bit, f float, d double): plain integers cost a fraction of wrapped ones."""
+    f = _FNS.get(name)
+    if f is None:
+        f = getattr(lib(), name)
+        f.argtypes = [{"p": _c.c_void_p, "i": _c.c_int, "l": _c.c_longlong, "f": _c.c_float, "d": _c.c_double}[c] for c in spec]
+        _FNS[name] = f
+    return f
+
+
+def _stream() -> int:
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _same_device(first: torch.Tensor, *others) -> None:
+    """All of a call's tensors live on the current device: the kernels launch there."""
+    dev = first.device
+    if dev.type != "cuda" or dev.index != torch.cuda.current_device() or any(t is not None and t.device != dev for t in others):
+        raise ValueError("the tensors of a call live on the current CUDA device")
+
+
+def _kv4_dims(k_cache, v_cache, hkv: int, dim: int) -> int:
+    """Block size of a pair of 4-bit caches the kernels can address."""
+    bs = ref.kv4_block_size(k_cache, dim)
+    if dim not in KV4_DIMS:
+        raise ValueError(f"4-bit rows on the GPU: head sizes {KV4_DIMS}, not {dim}")
+    if v_cache.dtype != torch.uint8 or v_cache.shape != k_cache.shape or k_cache.shape[1] != hkv:
+        raise ValueError(f"4-bit keys and values come in caches of one shape, of {hkv} kv heads")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()) or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+        raise ValueError("4-bit caches are contiguous and aligned to 16 bytes")
+    return bs
+
+
+def _slots_of(slot_mapping, T: int):
+    slots = _i64c(slot_mapping)
+    if slots.numel() != T:
+        raise ValueError(f"{slots.numel()} cache slots for {T} tokens")
+    return slots
+
+
+def _kv4_store(k_cache, v_cache, slot_mapping, k, v) -> None:
+    T, hkv, dim = k.shape
+    bs = _kv4_dims(k_cache, v_cache, hkv, dim)
+    if v.shape != k.shape or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise ValueError("4-bit rows are made of bf16 keys and values of one shape")
+    _same_device(k, v, k_cache, v_cache, slot_mapping)
+    if T == 0:
+        return
+    al = dim // 32                       # elements a lane loads at once
+    k2, v2 = (t if t.stride(2) == 1 and t.stride(1) == dim and t.stride(0) % al == 0 and t.data_ptr() % (2 * al) == 0
+              else t.clone(memory_format=torch.contiguous_format) for t in (k, v))
+    slots = _slots_of(slot_mapping, T)
+    _ck(_fn("ne_kv4_store", "ppllpppliiiip")(
+        k2.data_ptr(), v2.data_ptr(), k2.stride(0), v2.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), k_cache.shape[0] * bs, T, hkv, dim, bs,
+        _stream()), "ne_kv4_store")
+
+
+def gqa_kv_gather(k_cache, v_cache, slots, dim):
+    """One kernel: a thread per word of eight dims of a key row and its value row."""
+    T, hkv = slots.numel(), k_cache.shape[1]
+    bs = _kv4_dims(k_cache, v_cache, hkv, dim)
+    _same_device(k_cache, v_cache, slots)
+    k, v = (torch.empty(T, hkv, dim, dtype=torch.bfloat16, device=k_cache.device) for _ in range(2))
+    if T:
+        _ck(_fn("ne_kv4_gather", "ppplppiiiip")(k_cache.data_ptr(), v_cache.data_ptr(), _i64c(slots).data_ptr(), k_cache.shape[0] * bs, k.data_ptr(), v.data_ptr(), T, hkv, dim,
+                                                bs, _stream()), "ne_kv4_gather")
+    return k, v
+
+
+def _gqa_rows(qkv, hq, hkv, hd, q_norm_w, k_norm_w, eps, unit_offset, positions, rope_cache, k_cache, v_cache, slot_mapping, sections, interleaved):
+    T = qkv.shape[0]
+    int4 = k_cache.dtype == torch.uint8
+    if hd not in KV4_DIMS:
+        raise ValueError(f"positions on several axes and 4-bit rows on the GPU: head sizes {KV4_DIMS}, not {hd}")
+    if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != (hq + 2 * hkv) * hd:
+        raise ValueError(f"qkv is bf16 [T, {(hq + 2 * hkv) * hd}], not {qkv.dtype} {list(qkv.shape)}")
+    if rope_cache.dtype != torch.float32 or not rope_cache.is_contiguous() or rope_cache.dim() != 2 or rope_cache.shape[1] != hd:
+        raise ValueError(f"the rotary table is fp32 [positions, {hd}], contiguous")
+    if int4:
+        bs = _kv4_dims(k_cache, v_cache, hkv, hd)
+        rows = k_cache.shape[0] * bs
+    else:
+        bs, rows = 1, k_cache.shape[0] * k_cache.shape[1]
+        if any(c.dtype != torch.bfloat16 or not c.is_contiguous() or c.data_ptr() % 16 or c.shape != k_cache.shape or tuple(c.shape[2:]) != (hkv, hd) for c in (k_cache, v_cache)):
+            raise ValueError(f"caches: contiguous bf16 [blocks, block_size, {hkv}, {hd}] or 4-bit pages")
+    if sections is None:
+        sec = (hd // 2,)
+        if positions.numel() != T:
+            raise ValueError(f"{positions.numel()} positions for {T} tokens")
+    else:
+        sec = tuple(int(n) for n in sections)
+        if sum(sec) != hd // 2 or min(sec) < 0 or not 1 <= len(sec) <= 4:
+            raise ValueError(f"sections {list(sec)}: one to four axes whose angles add up to half a head, {hd // 2}")
+        if tuple(positions.shape) != (len(sec), T):
+            raise ValueError(f"positions {list(positions.shape)}: one row per axis of sections {list(sec)}")
+    _same_device(qkv, positions, rope_cache, k_cache, v_cache, slot_mapping, q_norm_w, k_norm_w)
+    q = torch.empty(T, hq, hd, dtype=torch.bfloat16, device=qkv.device)
+    slots = _slots_of(slot_mapping, T)
+    if T == 0:
+        return q
+    al = hd // 32
+    if qkv.stride(1) != 1 or qkv.stride(0) % al or qkv.data_ptr() % (2 * al):
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+    norms = []
+    for w in (q_norm_w, k_norm_w):
+        if w is not None and w.numel() != hd:
+            raise ValueError(f"norm weights have {hd} values")
+        w = None if w is None else w.to(torch.bfloat16).contiguous()
+        norms.append(w if w is None or w.data_ptr() % (2 * al) == 0 else w.clone())
+    pos = positions if positions.dtype == torch.int64 and positions.stride(-1) == 1 else positions.long().contiguous()
+    heads = hq + 2 * hkv
+    chunk = 1
+    _ck(_fn("ne_gqa_rows", "pliiippdfplpiipippppliiiip")(
+        qkv.data_ptr(), qkv.stride(0), hq, hkv, hd, 0 if norms[0] is None else norms[0].data_ptr(), 0 if norms[1] is None else norms[1].data_ptr(), float(eps),
+        1.0 if unit_offset else 0.0, pos.data_ptr(), pos.stride(0) if sections is not None else 0, rope_cache.data_ptr(), rope_cache.shape[0], len(sec),
+        (_c.c_int * len(sec))(*sec), 1 if interleaved else 0, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), rows, bs, 1 if int4 else 0, chunk, T,
+        _stream()), "ne_gqa_rows")
+    return q
+
+
+def kv4_expand(k_cache, v_cache, block_tables, context_lens, dim: int):
+    """The contexts of all sequences as bf16 caches of 64-token pages of their own: (k, v [B * width, 64, Hkv, dim], block tables [B, width], context lengths).
+    A context is cut off where its block table ends, a page outside the cache reads as zeros."""
+    hkv = k_cache.shape[1]
+    bs = _kv4_dims(k_cache, v_cache, hkv, dim)
+    B, W = block_tables.shape
+    width = max(1, -(-W * bs // 64))
+    k, v = (torch.empty(B * width, 64, hkv, dim, dtype=torch.bfloat16, device=k_cache.device) for _ in range(2))
+    bt = torch.empty(B, width, dtype=torch.int32, device=k_cache.device)
+    cl = torch.empty(B, dtype=torch.int32, device=k_cache.device)
+    _ck(_fn("ne_kv4_expand", "ppipli" + "piippppiiip")(k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], block_tables.data_ptr(), block_tables.stride(0), W,
+                                                      context_lens.data_ptr(), B, width, k.data_ptr(), v.data_ptr(), bt.data_ptr(), cl.data_ptr(), hkv, dim, bs, _stream()),
+        "ne_kv4_expand")
+    return k, v, bt, cl
+
+
+def step_tables(q_lens, seq_lens, block_ids, block_offsets, block_size, num_tokens, max_blocks, rows=None, pad_len=1, scratch_block=-1, out=None):
+    """One launch; every tensor int32 (other integers are converted)."""
+    B = q_lens.numel()
+    rows = ref._step_sizes(B, block_size, num_tokens, max_blocks, rows, pad_len, scratch_block)
+    if seq_lens.numel() != B or block_offsets.numel() != B + 1:
+        raise ValueError("step_tables: one length per sequence and one offset more")
+    if rows > 12000:
+        raise ValueError("step_tables: at most 12000 rows")
+    _same_device(q_lens, seq_lens, block_ids, block_offsets)
+    dev = q_lens.device
+    q, n, ids, off = (t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous() for t in (q_lens, seq_lens, block_ids, block_offsets))
+    sizes = [(rows + 1,), (rows,), (num_tokens,), (num_tokens,), (rows, max_blocks), (rows,)]
+    if out is None:
+        i32, i64 = dict(dtype=torch.int32, device=dev), dict(dtype=torch.int64, device=dev)
+        made = StepTables(torch.empty(rows + 1, **i32), torch.empty(rows, **i32), torch.empty(num_tokens, **i64), torch.empty(num_tokens, **i64),
+                          torch.empty(rows, max_blocks, **i32), torch.empty(rows, **i32))
+    else:
+        ref._check_step_out(out, sizes)
+        _same_device(q_lens, *out)
+        made = StepTables(*(o[tuple(slice(k) for k in size)] for o, size in zip(out, sizes)))
+    _ck(_fn("ne_step_tables", "pppp" + "iiiiiiii" + "ppppp" + "lpp")(
+        q.data_ptr(), n.data_ptr(), ids.data_ptr(), off.data_ptr(), B, rows, ids.numel(), int(block_size), int(num_tokens), int(max_blocks), int(pad_len), int(scratch_block),
+        made.cu_seqlens_q.data_ptr(), made.context_lens.data_ptr(), made.positions.data_ptr(), made.slot_mapping.data_ptr(), made.block_tables.data_ptr(),
+        made.block_tables.stride(0) if rows else int(max_blocks), made.last_token_indices.data_ptr(), _stream()), "ne_step_tables")
+    return made
 
 
 # ---- MoE -----------------------------------------------------------------------------------------

@@ -232,6 +232,8 @@ def gqa_attention_paged(q, k_cache, v_cache, block_tables, cu_seqlens_q, context
     """`window` > 0: every query sees only its last `window` key positions (sliding-window layers).  bf16 caches of 64-token pages: tensor cores.  Those
     layers, and head sizes other than 128, keep their probabilities in 32-bit (two bf16 terms); other caches run on the generic kernel."""
     T, Hq, D = q.shape
+    if k_cache.dtype == torch.uint8:
+        return _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale, window)
     Hkv = k_cache.shape[2]
     lib = _k.lib()
     bt, cu, cl = _i32(block_tables), _i32(cu_seqlens_q), _i32(context_lens)
@@ -277,6 +279,60 @@ def gqa_attention_paged(q, k_cache, v_cache, block_tables, cu_seqlens_q, context
                                _k._p(cu), _k._p(cl), _c.c_int(cl.numel()), _k._p(None), _c.c_int(0), _k._p(out), _c.c_longlong(Hq * D), _c.c_int(D),
                                _k._p(None), _c.c_int(T), _c.c_int(Hq), _c.c_int(D), _c.c_int(D), _c.c_float(scale), _c.c_int(0), _c.c_int(max(0, int(window))), _c.c_int(0), _k._st()),
            "ne_attn_generic")
+    return out
+
+
+INT4_CALLS = [0]             # launches of the kernel that reads 4-bit pages itself
+
+
+def _int4_splits(ctas: int, tiles: int) -> int:
+    """Key slices of the 4-bit kernel."""
+    if ctas >= _sms():
+        return 1
+    return max(1, min(_sms() // ctas, tiles // 4, 32))
+
+
+def _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale, window: int):
+    """4-bit pages: a kernel that unpacks them in registers for steps of few query rows per key, the tensor-core kernels over pages expanded to bf16 for others."""
+    T, Hq, D = q.shape
+    Hkv, bs = _k.ref.check_kv4(q, k_cache, v_cache)
+    _k._kv4_dims(k_cache, v_cache, Hkv, D)
+    if D == 32 or not (bs in (16, 32) or bs % 64 == 0):
+        raise ValueError(f"attention over 4-bit pages on the GPU: head sizes 64, 128 and 256, pages of 16, 32 or a multiple of 64 tokens, not {D} and {bs}")
+    if not scale > 0:
+        raise ValueError("the scale of the scores is positive")
+    bt, cu, cl = _i32(block_tables), _i32(cu_seqlens_q), _i32(context_lens)
+    B = cl.numel()
+    if bt.dim() != 2 or bt.shape[0] < B or cu.numel() != B + 1:
+        raise ValueError("one block table row per sequence, and one query boundary more")
+    _k._same_device(q, k_cache, v_cache, bt, cu, cl)
+    out = torch.empty(T, Hq, D, dtype=torch.bfloat16, device=q.device)
+    if T == 0:
+        return out
+    if B == 0 or bt.shape[1] == 0:
+        return out.zero_()
+    q = q if q.dtype == torch.bfloat16 and q.stride(2) == 1 and q.stride(1) == D and q.stride(0) % 4 == 0 and q.data_ptr() % 8 == 0 else \
+        q.to(torch.bfloat16).clone(memory_format=torch.contiguous_format)
+    g = Hq // Hkv
+    tq = max(1, 16 // g)
+    if T * g >= 128 * B and (g % 4 == 0 or g == 1 and Hq % 4 == 0) and g <= 128:
+        k, v, bt, cl = _k.kv4_expand(k_cache, v_cache, bt, cl, D)
+        return gqa_attention_paged(q, k, v, bt, cu, cl, scale, window)
+    tiles = min(T, T // tq + B)
+    ctas = tiles * Hkv * -(-g // 16)
+    keys = bt.shape[1] * bs if window <= 0 else min(bt.shape[1] * bs, window + tq + 62)
+    S = _int4_splits(ctas, -(-keys // 64))
+    part = lse2 = None
+    if S > 1:
+        part = torch.empty(S, T, Hq, D, dtype=torch.float32, device=q.device)
+        lse2 = torch.empty(S, T, Hq, dtype=torch.float32, device=q.device)
+    _k._ck(_k._fn("ne_gqa_int4", "plppiipli" + "ppi" + "iiiiiii" + "f" + "pppp")(
+        q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], bs, bt.data_ptr(), bt.stride(0), bt.shape[1], cu.data_ptr(), cl.data_ptr(), B,
+        T, Hq, Hkv, D, tiles, S, max(0, int(window)), scale, out.data_ptr(), 0 if part is None else part.data_ptr(), 0 if lse2 is None else lse2.data_ptr(), _k._stream()),
+        "ne_gqa_int4")
+    INT4_CALLS[0] += 1
+    if S > 1:
+        _k._ck(_k.lib().ne_attn_merge(_k._p(part), _k._p(lse2), _k._p(out), _c.c_int(S), _c.c_longlong(T * Hq), _c.c_int(D), _c.c_int(D), _k._st()), "ne_attn_merge")
     return out
 
 
