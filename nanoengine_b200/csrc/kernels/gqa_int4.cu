@@ -2,33 +2,179 @@
 //
 //   softmax(q k^T scale) v with k = (c - 8) s of 4-bit codes, a scale per 32 dims; causal, optionally the last `window` keys only
 //
-// Bound by HBM: D/2 + D/32 bytes a key row, 17/64 of bf16.  One CTA = one KV head x one tile of up to 16 (token, head of the group) rows of one sequence
-// x one slice of its keys; its warps take tiles of 64 keys in turn, each with a ring of bulk copies of its own (no barrier among warps until the end).
-// A key is unpacked once, in registers, straight into the fragments of mma.m16n8k16: a lane owns a contiguous quarter of a key row and an eighth of a value
-// row, the dims of a step of the product and the keys of a step of the second one are permuted to match (query rows and probabilities follow).  tcgen05
-// would want the unpacked tile in shared memory or TMEM: 16 rows fill an eighth of its M = 128, and the 64 KB of bf16 a tile of 64 keys would be written and
-// read there is seven times what is read from HBM.  Portions with many rows per key run on the tensor-core prompt kernel over expanded pages instead.
+// Bound by HBM: D/2 + D/32 bytes a key row, 17/64 of bf16.  A unit of work is a tile of 64 keys (32 for heads of 256) for up to 16 (token, head of the
+// group) rows of one sequence and KV head.  The units of the whole batch, laid end to end, are cut into equal shares, one per warp that fits the GPU:
+// ragged contexts keep no SM waiting, whatever their number, and no warp waits for another.  A warp walks its share with a ring of bulk copies of its own.
+// Where a share cuts a row tile, the pieces are written as 32-bit partial results, two places per warp, and a second kernel joins the pieces of every
+// tile that a cut runs through.
 //
-// Unpacked values (c - 8) s are exact in bf16, scores, maxima, sums and results are 32-bit, probabilities enter the second product as bf16 (2^-9 each) and
-// the sum takes them as rounded.  Every byte stands for a finite value, so a masked key (probability 0) adds nothing whatever its page holds.
+// A key is unpacked once, in registers, straight into the fragments of mma.m16n8k16: a lane owns a contiguous quarter of a key row and an eighth of a value
+// row; the dims of a step of the first product and the keys of a step of the second are permuted to match (query rows and probabilities follow).  tcgen05
+// would want the unpacked tile in shared memory: 16 rows fill an eighth of its M = 128, and the 32 KB of bf16 that a tile of 64 keys becomes would cross
+// shared memory twice, which takes longer than its 8.5 KB take to come from HBM.  Portions with many rows per key run on the tensor-core prompt kernel over
+// expanded pages instead.
+//
+// A masked nibble is a bf16 pair of subnormals c 2^-133 (16 c 2^-133 for the upper nibble of a byte), so that one fused multiply-add per pair gives
+// (c - 8) s 2^-24, exactly; the 2^24 goes into the softmax scale and the last division.  Scores, maxima, sums and results are 32-bit, probabilities enter
+// the second product as bf16 (2^-9 each) and their sum is a column of ones of the same product.  Every byte stands for a finite value, so a masked key
+// (probability 0) adds nothing whatever its page holds.
 #include "kv4.cuh"
-#include "seq_tile.cuh"
 
 namespace ne {
 
 constexpr int kKernelI4 = 31;
-constexpr int kTileKeys = 64;
+constexpr int kI4Warps = 4, kI4Threads = 32 * kI4Warps;
 
 struct I4Args {
   const __nv_bfloat16* q; long long q_ld;              // [T, Hq, D], rows q_ld apart
   const uint8_t* k; const uint8_t* v; int num_blocks, block_size;
   const int* block_tables; long long bt_ld; int bt_width;
   const int* cu_seqlens_q; const int* context_lens; int num_seqs;
-  int T, Hq, Hkv, g, tq, head_tiles, splits, window;   // tq tokens x min(g, 16) heads a tile; head_tiles = ceil(g / 16)
+  int T, Hq, Hkv, g, tq, head_tiles, window, shares;   // tq tokens x min(g, 16) heads a row tile; head_tiles = ceil(g / 16)
   float scale_log2;
-  __nv_bfloat16* out;                                  // [T, Hq, D] (splits == 1)
-  float* part; float* lse2;                            // [splits, T, Hq, D], [splits, T, Hq] (splits > 1)
+  __nv_bfloat16* out;                                  // [T, Hq, D]
+  float* part; float* lse2;                            // [shares, 2, 16, D], [shares, 2, 16]
+  int4* cuts;                                          // [1 + row tiles]: how many row tiles there are; what the join needs of each
 };
+
+template <int D> struct I4Geo {
+  static constexpr int keys = D == 256 ? 32 : 64;                       // of a tile
+  static constexpr int slots = D == 256 ? 2 : 3;                        // of a warp's ring
+  static constexpr int ctas = D == 64 ? 3 : 2;                          // resident per SM
+  static constexpr int row = D / 2, srow = D / 32;                      // bytes of a row's codes and scales
+  static constexpr int codes = keys * row, half = codes + keys * srow, stage = 2 * half;
+  static constexpr int words = D / 32;                                  // words of a key row a lane owns (a quarter of the row)
+  static constexpr int vwords = D / 64;                                 // words of a value row a lane owns (an eighth)
+  static constexpr int ks = D / 16;                                     // k steps of the first product
+  static constexpr int nt = D / 8;                                      // column tiles of the second one
+  static constexpr bool q_regs = D <= 128;                              // query fragments in registers, else in shared memory
+  static constexpr int warp_bytes = slots * stage + (q_regs ? 0 : ks * 512);
+  static constexpr int smem = kI4Warps * warp_bytes;
+};
+
+// ---- shares: the units of all sequences end to end ----
+struct I4Seq { int q_beg, q_len, ctx, first, per_tile, tiles; };        // first: first tile of keys; per_tile: units of a (row tile, head)
+
+template <int KEYS> __device__ __forceinline__ I4Seq i4_seq(const I4Args& a, int q_beg, int q_end, int ctx) {
+  I4Seq s;
+  s.q_beg = q_beg;
+  s.q_len = max(0, q_end - q_beg);
+  s.ctx = (int)max(0ll, min((long long)ctx, (long long)a.bt_width * a.block_size));
+  const int first_key = a.window > 0 ? max(0, s.ctx - s.q_len - a.window + 1) : 0;
+  s.first = first_key / KEYS;
+  s.per_tile = max(1, (s.ctx + KEYS - 1) / KEYS - s.first);              // a tile that sees no key still writes its zeros
+  s.tiles = (s.q_len + a.tq - 1) / a.tq;
+  return s;
+}
+template <int KEYS> __device__ __forceinline__ I4Seq i4_load(const I4Args& a, int i) {
+  return i4_seq<KEYS>(a, a.cu_seqlens_q[i], a.cu_seqlens_q[i + 1], a.context_lens[i]);
+}
+
+// Units of a share: equal ones, but no less than two
+__device__ __forceinline__ int i4_share(int total, int shares) { return max((total + shares - 1) / shares, 2); }
+
+constexpr int kI4MaxSlots = 3;
+struct I4Shared {
+  uint64_t bar[kI4Warps * kI4MaxSlots];                                  // a slot's tile has landed
+  uint32_t bad[kI4Warps * kI4MaxSlots];                                  // pieces of it whose page lies outside the cache
+  int abort, warp[2 * kI4Warps];
+  int4 start[kI4Warps];                                                  // sequence that a warp's share starts in; units and row tiles in front of it
+  int beg[kI4Threads], end[kI4Threads], ctx[kI4Threads];                 // what the sequences from the first of these on are
+};
+
+// Totals (units, row tiles), and where the shares of this CTA's warps start.  All threads of the CTA, each with a run of sequences.
+template <int KEYS> __device__ __forceinline__ int2 i4_plan(const I4Args& a, I4Shared& sh, int& share) {
+  const int run = (a.num_seqs + kI4Threads - 1) / kI4Threads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int s0 = threadIdx.x * run, s1 = min(a.num_seqs, s0 + run), heads = a.Hkv * a.head_tiles;
+  int mine = 0, tiles = 0;
+  for (int i = s0; i < s1; i++) {
+    const I4Seq s = i4_load<KEYS>(a, i);
+    tiles += s.tiles * heads;
+    mine += s.tiles * heads * s.per_tile;
+  }
+  int incl = mine, incl_t = tiles;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, o), t = __shfl_up_sync(0xffffffffu, incl_t, o);
+    if (lane >= o) { incl += v; incl_t += t; }
+  }
+  if (lane == 31) { sh.warp[warp] = incl; sh.warp[kI4Warps + warp] = incl_t; }
+  __syncthreads();
+  int before = incl - mine, before_t = incl_t - tiles;
+  int2 total = make_int2(0, 0);
+#pragma unroll
+  for (int w = 0; w < kI4Warps; w++) {
+    if (w < warp) { before += sh.warp[w]; before_t += sh.warp[kI4Warps + w]; }
+    total.x += sh.warp[w]; total.y += sh.warp[kI4Warps + w];
+  }
+  share = i4_share(total.x, a.shares);
+#pragma unroll
+  for (int w = 0; w < kI4Warps; w++) {                                   // the thread whose run a share starts in finds the sequence
+    const long long u = ((long long)blockIdx.x * kI4Warps + w) * share;
+    if (u < before || u >= before + mine) continue;
+    int base = before, t = before_t;
+    for (int i = s0;; i++) {
+      const I4Seq s = i4_load<KEYS>(a, i);
+      const int n = s.tiles * heads;
+      if (u < base + n * s.per_tile || i + 1 >= s1) { sh.start[w] = make_int4(i, base, t, 0); break; }
+      base += n * s.per_tile;
+      t += n;
+    }
+  }
+  __syncthreads();
+  return total;
+}
+
+// A piece of work: units [unit, unit + units) of one (row tile, head)
+struct I4Piece {
+  I4Seq s; int seq, tile, hkv, ht, index, unit, units;                   // ht: tile of the group's heads; index: of this row tile among all
+  int gh, head0, tok0, n_tok, base_limit, t_begin, t_end;                // t_begin .. t_end: its tiles of keys that any row sees
+};
+template <int KEYS> __device__ __forceinline__ void i4_fill(const I4Args& a, I4Piece& p, int left) {
+  p.units = min(p.s.per_tile - p.unit, left);
+  p.gh = min(a.g - p.ht * 16, 16);
+  p.head0 = p.hkv * a.g + p.ht * 16;
+  p.tok0 = p.s.q_beg + p.tile * a.tq;
+  p.n_tok = p.tok0 < 0 ? 0 : min(min(a.tq, p.s.q_len - p.tile * a.tq), a.T - p.tok0);
+  p.base_limit = p.s.ctx - p.s.q_len + p.tile * a.tq;                    // last key the tile's first token sees
+  const int max_limit = p.base_limit + p.n_tok - 1;
+  const int low = a.window > 0 ? max(0, p.base_limit - a.window + 1) / KEYS : 0;
+  p.t_begin = max(p.s.first + p.unit, low);
+  p.t_end = p.n_tok > 0 ? min(p.s.first + p.unit + p.units, max_limit >= 0 ? max_limit / KEYS + 1 : 0) : 0;
+}
+// the piece that starts at unit u, in the sequence that `at` names; `left` units of the share remain
+template <int KEYS> __device__ __forceinline__ I4Piece i4_first(const I4Args& a, const int4& at, int u, int left) {
+  I4Piece p;
+  p.seq = at.x;
+  p.s = i4_load<KEYS>(a, p.seq);
+  const int heads = a.Hkv * a.head_tiles, th = (u - at.y) / p.s.per_tile, head = th % heads;
+  p.unit = u - at.y - th * p.s.per_tile;
+  p.index = at.z + th;
+  p.tile = th / heads;
+  p.hkv = head / a.head_tiles;
+  p.ht = head - p.hkv * a.head_tiles;
+  i4_fill<KEYS>(a, p, left);
+  return p;
+}
+// the piece behind p
+template <int KEYS> __device__ __forceinline__ void i4_next(const I4Args& a, const I4Shared& sh, I4Piece& p, int left) {
+  p.unit = 0;
+  p.index++;
+  if (++p.ht == a.head_tiles) {
+    p.ht = 0;
+    if (++p.hkv == a.Hkv) {
+      p.hkv = 0;
+      if (++p.tile == p.s.tiles) {
+        p.tile = 0;
+        do {
+          const int i = ++p.seq - sh.start[0].x;
+          p.s = i < kI4Threads ? i4_seq<KEYS>(a, sh.beg[i], sh.end[i], sh.ctx[i]) : i4_load<KEYS>(a, p.seq);
+        } while (p.s.tiles == 0 && p.seq + 1 < a.num_seqs);
+      }
+    }
+  }
+  i4_fill<KEYS>(a, p, left);
+}
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
@@ -38,285 +184,378 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int D> struct I4Geo {
-  static constexpr int row = D / 2, srow = D / 32;                      // bytes of a row's codes and scales
-  static constexpr int codes = kTileKeys * row, half = codes + kTileKeys * srow, stage = 2 * half;
-  static constexpr int words = D / 32;                                  // words of a key row a lane owns (a quarter of the row)
-  static constexpr int vwords = D / 64;                                 // words of a value row a lane owns (an eighth)
-  static constexpr int ks = D / 16;                                     // k steps of the first product
-  static constexpr int nt = D / 8;                                      // column tiles of the second one
-};
+// Multipliers of one scale (or of a pair of scales) as bf16 pairs, from (byte << 4) in both halves: s 2^109 for the lower nibble of a byte, s 2^105 for the
+// upper one, -8 s 2^-24.  None leaves bf16's exponents.  (Two of them by exact products: the integer pipe is the busier one.)
+struct I4Scale { uint32_t lo, hi, z; };
+__device__ __forceinline__ I4Scale i4_scale(uint32_t b4) {
+  const uint32_t lo = b4 + 0x6E006E00u;
+  return {lo, hmul2_bf16(lo, 0x3D803D80u), hmul2_bf16(lo, 0x80088008u)};
+}
+__device__ __forceinline__ uint32_t i4_lower(uint32_t w, const I4Scale& s) { return hfma2_bf16(w & 0x000F000Fu, s.lo, s.z); }
+__device__ __forceinline__ uint32_t i4_upper(uint32_t w, const I4Scale& s) { return hfma2_bf16(w & 0x00F000F0u, s.hi, s.z); }
 
-template <int D, int W, int ST>
-__global__ void __launch_bounds__(W * 32, 1) gqa_int4_kernel(const I4Args a) {
+template <int D, bool kPlain>
+__global__ void __launch_bounds__(kI4Threads, I4Geo<D>::ctas) gqa_int4_kernel(const I4Args a) {
   using G = I4Geo<D>;
+  constexpr int ST = G::slots, JT = G::keys / 8;                         // JT: column tiles of the scores
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t s_bar[W * ST];
-  __shared__ uint32_t s_bad[W * ST];                                     // pieces of a slot whose page lies outside the cache
-  __shared__ int s_tile[2];
-  __shared__ int s_abort;
-  __shared__ float s_m[W][16], s_l[W][16];
+  __shared__ I4Shared sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c = lane & 3, n = lane >> 2;                                 // fragment coordinates: column pair, row
   if (threadIdx.x == 0) {
-    s_abort = 0;
-    for (int i = 0; i < W * ST; i++) mbar_init(smem_u32(&s_bar[i]), 1);
+    sh.abort = 0;
+    for (int i = 0; i < kI4Warps * ST; i++) mbar_init(smem_u32(&sh.bar[i]), 1);
     mbar_fence_init();
   }
   pdl_wait(); pdl_trigger();
-  if (warp == 0) {
-    int seq, tok;
-    find_seq_tile(a.cu_seqlens_q, a.num_seqs, a.tq, blockIdx.x, seq, tok);
-    if (lane == 0) { s_tile[0] = seq; s_tile[1] = tok; }
+  int share;
+  const int2 total = i4_plan<G::keys>(a, sh, share);                     // (its barriers also publish the initialised mbarriers)
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.cuts[0] = make_int4(total.y, 0, 0, 0);
+  if ((long long)blockIdx.x * kI4Warps * share >= total.x) return;
+  if (const int i = sh.start[0].x + threadIdx.x; i < a.num_seqs) {
+    sh.beg[threadIdx.x] = a.cu_seqlens_q[i]; sh.end[threadIdx.x] = a.cu_seqlens_q[i + 1]; sh.ctx[threadIdx.x] = a.context_lens[i];
   }
-  __syncthreads();
-  const int seq = s_tile[0], tok0 = s_tile[1];
-  if (seq < 0) return;
-  const int hkv = blockIdx.y / a.head_tiles, head0 = (blockIdx.y - hkv * a.head_tiles) * 16, split = blockIdx.z;
-  const int gh = min(a.g - head0, 16);                                   // heads of this tile
-  const int q_beg = a.cu_seqlens_q[seq], q_len = a.cu_seqlens_q[seq + 1] - q_beg;
-  const int n_tok = min(min(a.tq, q_beg + q_len - tok0), a.T - tok0);
-  if (n_tok <= 0 || tok0 < 0) return;
-  const int ctx = (int)min((long long)a.context_lens[seq], (long long)a.bt_width * a.block_size);
-  const int base_limit = ctx - q_len + (tok0 - q_beg);                   // last key the tile's first token sees
-  const int max_limit = base_limit + n_tok - 1;
-  const int first_key = a.window > 0 ? max(0, base_limit - a.window + 1) : 0;
-  int t_begin = 0, t_end = 0;                                            // this slice's tiles of 64 keys
-  if (max_limit >= first_key) {
-    const int lo = first_key / kTileKeys, total = max_limit / kTileKeys + 1 - lo, per = (total + a.splits - 1) / a.splits;
-    t_begin = lo + min(split * per, total);
-    t_end = lo + min((split + 1) * per, total);
-  }
-  const int* bt = a.block_tables + (long long)seq * a.bt_ld;
-  const int used_pages = (ctx + a.block_size - 1) / a.block_size;
-  const long long page_bytes = (long long)a.block_size * (G::row + G::srow);
-  uint8_t* ring = smem + warp * (ST * G::stage);
+  const int mine = blockIdx.x * kI4Warps + warp;                         // this warp's share
+  const long long u0 = (long long)mine * share;
+  int left = (int)min((long long)share, max(0ll, total.x - u0));         // units of it still to do
+  uint8_t* ring = smem + warp * G::warp_bytes;
+  uint64_t* bars = sh.bar + warp * ST;
+  const uint32_t page_bytes = (uint32_t)a.block_size * (G::row + G::srow), id_bytes = a.Hkv * page_bytes;      // of one head, of a page id
+  const bool one_page = a.block_size == G::keys;                         // a tile of keys is a page (kPlain: lies in one)
+  const float scale = a.scale_log2 * 16777216.f;
 
-  // this lane's two query rows (fragment rows n and n + 8): token and head
-  const int r0 = n, r1 = n + 8;
-  const int t0 = r0 / gh, t1 = r1 / gh;
-  const bool ok0 = t0 < n_tok, ok1 = t1 < n_tok;
-  const int hd0 = hkv * a.g + head0 + r0 % gh, hd1 = hkv * a.g + head0 + r1 % gh;
-  const int lim0 = ok0 ? base_limit + t0 : -1, lim1 = ok1 ? base_limit + t1 : -1;
-
-  uint32_t qa[G::ks][4];
-  {
-    const uint2* p0 = reinterpret_cast<const uint2*>(a.q + (long long)(tok0 + (ok0 ? t0 : 0)) * a.q_ld + (long long)hd0 * D + c * (D / 4));
-    const uint2* p1 = reinterpret_cast<const uint2*>(a.q + (long long)(tok0 + (ok1 ? t1 : 0)) * a.q_ld + (long long)hd1 * D + c * (D / 4));
-#pragma unroll
-    for (int ks = 0; ks < G::ks; ks++) {
-      const uint2 u0 = ok0 ? p0[ks] : make_uint2(0, 0), u1 = ok1 ? p1[ks] : make_uint2(0, 0);
-      qa[ks][0] = u0.x; qa[ks][1] = u1.x; qa[ks][2] = u0.y; qa[ks][3] = u1.y;
-    }
-  }
-
-  // copies of one tile into a slot: pieces of one page each; lane 0 only
-  const int piece = min(a.block_size, kTileKeys), pieces = kTileKeys / piece;
-  auto fetch = [&](int tile, int slot) {
-    const uint32_t bar = smem_u32(&s_bar[warp * ST + slot]), dst = smem_u32(ring + slot * G::stage);
-    int id[kTileKeys / 16];
-    uint32_t bytes = 0, bad = 0;
-#pragma unroll
-    for (int p = 0; p < kTileKeys / 16; p++) {
-      id[p] = -1;
-      if (p >= pieces) continue;
-      const int pg = (tile * kTileKeys + p * piece) / a.block_size;
-      if (pg >= used_pages) continue;                                    // behind the context: masked, whatever the slot holds
-      id[p] = bt[pg];
-      if (id[p] >= 0 && id[p] < a.num_blocks && NE_INDEX_OK(id[p], BK_CACHE_PAGES, kKernelI4, __LINE__)) bytes += 2 * piece * (G::row + G::srow);
-      else { id[p] = -1; bad |= 1u << p; }
-    }
-    s_bad[warp * ST + slot] = bad;                                       // seen by the others behind the barrier's phase
-    if (bytes) mbar_expect_tx(bar, bytes); else mbar_arrive(bar);
-#pragma unroll
-    for (int p = 0; p < kTileKeys / 16; p++) {
-      if (id[p] < 0) continue;
-      const int key = tile * kTileKeys + p * piece, tok = key % a.block_size;
-      const long long at = ((long long)id[p] * a.Hkv + hkv) * page_bytes;
-      if (a.block_size == kTileKeys) {                                   // a page is a tile: codes and scales in one piece
-        bulk_load(dst, a.k + at, G::half, bar);
-        bulk_load(dst + G::half, a.v + at, G::half, bar);
-      } else {
-        const long long sc = at + a.block_size * G::row + tok * G::srow;
-        const uint32_t d0 = dst + p * piece * G::row, d1 = dst + G::codes + p * piece * G::srow;
-        bulk_load(d0, a.k + at + tok * G::row, piece * G::row, bar);
-        bulk_load(d1, a.k + sc, piece * G::srow, bar);
-        bulk_load(d0 + G::half, a.v + at + tok * G::row, piece * G::row, bar);
-        bulk_load(d1 + G::half, a.v + sc, piece * G::srow, bar);
-      }
-    }
-  };
-
-  float o[G::nt][4];
-#pragma unroll
-  for (int i = 0; i < G::nt; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-
-  if (lane == 0)
-    for (int i = 0; i < ST; i++) if (t_begin + warp + i * W < t_end) fetch(t_begin + warp + i * W, i);
-  int slot = 0, phase = 0;
-  for (int tile = t_begin + warp; tile < t_end; tile += W) {
-    if (!mbar_wait(smem_u32(&s_bar[warp * ST + slot]), phase, (volatile int*)&s_abort, kKernelI4, 100 + slot)) break;
-    uint8_t* kt = ring + slot * G::stage;
-    const uint8_t* vt = kt + G::half;
-    if (const uint32_t bad = s_bad[warp * ST + slot]) {                  // pages outside the cache read as zeros: code 8
-      for (int p = 0; p < pieces; p++)
-        if (bad >> p & 1)
-          for (int i = lane; i < piece * G::row / 4; i += 32) {
-            reinterpret_cast<uint32_t*>(kt + p * piece * G::row)[i] = 0x88888888u;
-            reinterpret_cast<uint32_t*>(kt + G::half + p * piece * G::row)[i] = 0x88888888u;
+  // The copies of a tile of keys into a slot.  Pages outside the cache are marked; those behind the context stay masked, whatever the slot holds.
+  auto fetch = [&](const I4Piece& p, int tile, int slot, int id) {
+    const uint32_t bar = smem_u32(bars + slot), dst = smem_u32(ring) + slot * G::stage;
+    if constexpr (kPlain) {
+      if (lane == 0) {
+        const bool there = id >= 0 && id < a.num_blocks && NE_INDEX_OK(id, BK_CACHE_PAGES, kKernelI4, __LINE__);
+        sh.bad[warp * ST + slot] = !there;                               // seen by the others behind the barrier's phase
+        if (!there) mbar_arrive(bar);
+        else {
+          const unsigned long long at = (unsigned long long)(uint32_t)id * id_bytes + (uint32_t)p.hkv * page_bytes;
+          mbar_expect_tx(bar, G::stage);
+          if (one_page) {
+            bulk_load(dst, a.k + at, G::half, bar);
+            bulk_load(dst + G::half, a.v + at, G::half, bar);
+          } else {
+            const int tok = tile * G::keys % a.block_size, c0 = tok * G::row, s0 = a.block_size * G::row + tok * G::srow;
+            bulk_load(dst, a.k + at + c0, G::codes, bar);
+            bulk_load(dst + G::codes, a.k + at + s0, G::half - G::codes, bar);
+            bulk_load(dst + G::half, a.v + at + c0, G::codes, bar);
+            bulk_load(dst + G::half + G::codes, a.v + at + s0, G::half - G::codes, bar);
           }
-      __syncwarp();
-    }
-    // scores: column tile j = (kk, t) holds for fragment column 2 c' + e the key 16 kk + 4 (2 t + e) + (c' ^ e): neighbouring lanes read neighbouring rows
-    float s[8][4];
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-      const int key = 16 * (j >> 1) + 4 * (2 * (j & 1) + (n & 1)) + ((n >> 1) ^ (n & 1));
-      uint32_t w[G::words];
-      const uint8_t* src = kt + key * G::row + c * (G::row / 4);
-      if constexpr (D == 64) { const uint2 u = *reinterpret_cast<const uint2*>(src); w[0] = u.x; w[1] = u.y; }
-      else {
-#pragma unroll
-        for (int i = 0; i < G::words / 4; i++) {
-          const uint4 u = reinterpret_cast<const uint4*>(src)[i];
-          w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
         }
       }
-      const uint8_t* sp = kt + G::codes + key * G::srow;
-#pragma unroll
-      for (int i = 0; i < G::words; i++) {
-        uint32_t s2, z;
-        if (i % 4 == 0) {
-          s2 = kv4_scale_bits(sp[D == 64 ? c >> 1 : D == 128 ? c : 2 * c + i / 4]) * 0x00010001u;
-          z = kv4_minus24(s2);
-        }
-        mma_16816(s[j], qa[2 * i], kv4_pair<0>(w[i], s2, z), kv4_pair<1>(w[i], s2, z));
-        mma_16816(s[j], qa[2 * i + 1], kv4_pair<2>(w[i], s2, z), kv4_pair<3>(w[i], s2, z));
-      }
-    }
-    const int key0 = tile * kTileKeys;
-    if (key0 + kTileKeys - 1 > base_limit || (a.window > 0 && key0 <= max_limit - a.window)) {
-      const int low0 = a.window > 0 ? lim0 - a.window : -1, low1 = a.window > 0 ? lim1 - a.window : -1;
-#pragma unroll
-      for (int j = 0; j < 8; j++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const int key = key0 + 16 * (j >> 1) + 4 * (2 * (j & 1) + e) + (c ^ e);
-          if (key > lim0 || key <= low0) s[j][e] = -INFINITY;
-          if (key > lim1 || key <= low1) s[j][2 + e] = -INFINITY;
-        }
-    }
-    float x0 = -INFINITY, x1 = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      x0 = fmaxf(x0, fmaxf(s[j][0], s[j][1]));
-      x1 = fmaxf(x1, fmaxf(s[j][2], s[j][3]));
-    }
-#pragma unroll
-    for (int d = 1; d < 4; d <<= 1) {
-      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
-      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
-    }
-    x0 *= a.scale_log2; x1 *= a.scale_log2;
-    // the reference maximum moves only when a tile's exceeds it by more than 2^8
-    const bool up0 = x0 > m0 + 8.f || m0 == -INFINITY, up1 = x1 > m1 + 8.f || m1 == -INFINITY;
-    if (__any_sync(0xffffffffu, (up0 && x0 > m0) || (up1 && x1 > m1))) {
-      const float n0 = up0 ? fmaxf(m0, x0) : m0, n1 = up1 ? fmaxf(m1, x1) : m1;
-      const float f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - n0), f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - n1);
-      m0 = n0; m1 = n1; l0 *= f0; l1 *= f1;
-#pragma unroll
-      for (int i = 0; i < G::nt; i++) { o[i][0] *= f0; o[i][1] *= f0; o[i][2] *= f1; o[i][3] *= f1; }
-    }
-    const float z0 = m0 == -INFINITY ? 0.f : -m0, z1 = m1 == -INFINITY ? 0.f : -m1;
-#pragma unroll
-    for (int kk = 0; kk < 4; kk++) {
-      uint32_t p[4];
-#pragma unroll
-      for (int t = 0; t < 2; t++) {
-        const float (&v)[4] = s[2 * kk + t];
-        p[2 * t] = pack_bf16x2(exp2f(fmaf(v[0], a.scale_log2, z0)), exp2f(fmaf(v[1], a.scale_log2, z0)));
-        p[2 * t + 1] = pack_bf16x2(exp2f(fmaf(v[2], a.scale_log2, z1)), exp2f(fmaf(v[3], a.scale_log2, z1)));
-        const float2 e0 = unpack_bf16x2(p[2 * t]), e1 = unpack_bf16x2(p[2 * t + 1]);
-        l0 += e0.x + e0.y; l1 += e1.x + e1.y;
-      }
-      // values: this lane's four keys of the step, an eighth of each row
-      uint32_t w[4][G::vwords], sb[4];
-#pragma unroll
-      for (int u = 0; u < 4; u++) {
-        const int key = 16 * kk + 4 * u + (c ^ (u & 1));
-        const uint8_t* src = vt + key * G::row + n * (G::row / 8);
-        if constexpr (D == 64) w[u][0] = *reinterpret_cast<const uint32_t*>(src);
-        else if constexpr (D == 128) { const uint2 x = *reinterpret_cast<const uint2*>(src); w[u][0] = x.x; w[u][1] = x.y; }
-        else { const uint4 x = *reinterpret_cast<const uint4*>(src); w[u][0] = x.x; w[u][1] = x.y; w[u][2] = x.z; w[u][3] = x.w; }
-        sb[u] = vt[G::codes + key * G::srow + (D == 64 ? n >> 2 : D == 128 ? n >> 1 : n)];
-      }
-      const uint32_t sa2 = kv4_scale_bits(sb[0]) | kv4_scale_bits(sb[1]) << 16, sb2 = kv4_scale_bits(sb[2]) | kv4_scale_bits(sb[3]) << 16;
-      const uint32_t za = kv4_minus24(sa2), zb = kv4_minus24(sb2);
-#pragma unroll
-      for (int i = 0; i < G::vwords; i++) {
-        const uint32_t al = __byte_perm(w[0][i], w[1][i], 0x5410), ah = __byte_perm(w[0][i], w[1][i], 0x7632);
-        const uint32_t bl = __byte_perm(w[2][i], w[3][i], 0x5410), bh = __byte_perm(w[2][i], w[3][i], 0x7632);
-        mma_16816(o[8 * i + 0], p, kv4_pair<0>(al, sa2, za), kv4_pair<0>(bl, sb2, zb));
-        mma_16816(o[8 * i + 1], p, kv4_pair<0>(ah, sa2, za), kv4_pair<0>(bh, sb2, zb));
-        mma_16816(o[8 * i + 2], p, kv4_pair<1>(al, sa2, za), kv4_pair<1>(bl, sb2, zb));
-        mma_16816(o[8 * i + 3], p, kv4_pair<1>(ah, sa2, za), kv4_pair<1>(bh, sb2, zb));
-        mma_16816(o[8 * i + 4], p, kv4_pair<2>(al, sa2, za), kv4_pair<2>(bl, sb2, zb));
-        mma_16816(o[8 * i + 5], p, kv4_pair<2>(ah, sa2, za), kv4_pair<2>(bh, sb2, zb));
-        mma_16816(o[8 * i + 6], p, kv4_pair<3>(al, sa2, za), kv4_pair<3>(bl, sb2, zb));
-        mma_16816(o[8 * i + 7], p, kv4_pair<3>(ah, sa2, za), kv4_pair<3>(bh, sb2, zb));
-      }
+    } else {
+    // pages smaller than a tile: a lane copies each
+    const int bs = a.block_size, pg = tile * (G::keys / bs) + lane;
+    const bool seen = lane < G::keys / bs && pg < (p.s.ctx + bs - 1) / bs;
+    const int pid = seen ? a.block_tables[(long long)p.seq * a.bt_ld + pg] : -1;
+    const bool there = pid >= 0 && pid < a.num_blocks && NE_INDEX_OK(pid, BK_CACHE_PAGES, kKernelI4, __LINE__);
+    const unsigned all = __ballot_sync(0xffffffffu, there), bad = __ballot_sync(0xffffffffu, seen && !there);
+    if (lane == 0) {
+      sh.bad[warp * ST + slot] = bad;
+      if (all) mbar_expect_tx(bar, __popc(all) * 2 * bs * (G::row + G::srow)); else mbar_arrive(bar);
     }
     __syncwarp();
-    if (lane == 0 && tile + ST * W < t_end) fetch(tile + ST * W, slot);
-    if (++slot == ST) { slot = 0; phase ^= 1; }
-  }
+    if (there) {
+      const unsigned long long at = (unsigned long long)(uint32_t)pid * id_bytes + (uint32_t)p.hkv * page_bytes;
+      const uint32_t c0 = dst + lane * bs * G::row, s0 = dst + G::codes + lane * bs * G::srow;
+      bulk_load(c0, a.k + at, bs * G::row, bar);
+      bulk_load(s0, a.k + at + bs * G::row, bs * G::srow, bar);
+      bulk_load(c0 + G::half, a.v + at, bs * G::row, bar);
+      bulk_load(s0 + G::half, a.v + at + bs * G::row, bs * G::srow, bar);
+    }
+    }
+  };
+  // page of a tile of keys (its id is read one tile ahead of the copies)
+  auto page_of = [&](const I4Piece& p, int tile) {
+    return kPlain && tile < p.t_end ? a.block_tables[(long long)p.seq * a.bt_ld + (one_page ? tile : tile * G::keys / a.block_size)] : -1;
+  };
 
-  // join the warps: results and statistics meet in the ring's memory
+  I4Piece p;
+  if (left > 0) p = i4_first<G::keys>(a, sh.start[warp], (int)u0, left);
+  __syncthreads();                                                       // the table of sequences
+  if (left == 0) return;
+  int slot = 0, phase = 0;                                               // of the next tile to read
+#pragma unroll 1
+  for (int i = 0; i < ST; i++) if (p.t_begin + i < p.t_end) fetch(p, p.t_begin + i, i, page_of(p, p.t_begin + i));
+
+  while (true) {
+    const int n_tok = p.n_tok, gh = p.gh, head0 = p.head0, tok0 = p.tok0, base_limit = p.base_limit, max_limit = p.base_limit + p.n_tok - 1;
+    int id = page_of(p, p.t_begin + ST);
+
+    // this lane's two query rows (fragment rows n and n + 8): token and head
+    const int t0 = gh == 16 ? 0 : n / gh, t1 = gh == 16 ? 0 : (n + 8) / gh, h0 = n - t0 * gh, h1 = n + 8 - t1 * gh;
+    const bool ok0 = t0 < n_tok, ok1 = t1 < n_tok;
+    const int lim0 = ok0 ? base_limit + t0 : -1, lim1 = ok1 ? base_limit + t1 : -1;
+    uint32_t qa[G::q_regs ? G::ks : 1][4];
+    uint4* sq = reinterpret_cast<uint4*>(ring + ST * G::stage);
+    {
+      const uint2* p0 = reinterpret_cast<const uint2*>(a.q + (long long)(tok0 + (ok0 ? t0 : 0)) * a.q_ld + (long long)(head0 + h0) * D + c * (D / 4));
+      const uint2* p1 = reinterpret_cast<const uint2*>(a.q + (long long)(tok0 + (ok1 ? t1 : 0)) * a.q_ld + (long long)(head0 + h1) * D + c * (D / 4));
+      if constexpr (G::q_regs) {
+        // the products want the four words of a step in neighbouring registers, the loads pairs of them: without an operation in between, every product moves them
+        const uint32_t nil = (uint32_t)a.shares >> 31;
 #pragma unroll
-  for (int d = 1; d < 4; d <<= 1) { l0 += __shfl_xor_sync(0xffffffffu, l0, d); l1 += __shfl_xor_sync(0xffffffffu, l1, d); }
-  __syncthreads();                                                       // every warp's last tile has been read
-  if (s_abort) {                                                         // copies may still be in flight: let them land before the block ends
-    if (threadIdx.x == 0) for (int i = 0; i < 2000; i++) __nanosleep(1000);
+        for (int ks = 0; ks < G::ks; ks++) {
+          const uint2 x0 = ok0 ? p0[ks] : make_uint2(0, 0), x1 = ok1 ? p1[ks] : make_uint2(0, 0);
+          qa[ks][0] = x0.x ^ nil; qa[ks][1] = x1.x ^ nil; qa[ks][2] = x0.y ^ nil; qa[ks][3] = x1.y ^ nil;
+        }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < G::ks; ks++) {
+          const uint2 x0 = ok0 ? p0[ks] : make_uint2(0, 0), x1 = ok1 ? p1[ks] : make_uint2(0, 0);
+          sq[ks * 32 + lane] = make_uint4(x0.x, x1.x, x0.y, x1.y);
+        }
+        __syncwarp();
+      }
+    }
+
+    float o[G::nt][4], l[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < G::nt; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY;
+
+#pragma unroll 1
+    for (int tile = p.t_begin; tile < p.t_end; tile++) {
+      const uint8_t* kt = ring + slot * G::stage;
+      const uint8_t* vt = kt + G::half;
+      const bool landed = mbar_wait(smem_u32(bars + slot), phase, (volatile int*)&sh.abort, kKernelI4, 100 + slot, 1);
+      if (!__all_sync(0xffffffffu, landed)) {                            // a copy has not come: let the others land before the block's memory goes
+        for (int i = 0; i < 2000; i++) __nanosleep(1000);
+        return;
+      }
+      if (const uint32_t bad = sh.bad[warp * ST + slot]) {               // pages outside the cache read as zeros: code 8
+        const int piece = min(a.block_size, G::keys);
+        for (int q = 0; q < G::keys / piece; q++)
+          if (bad >> q & 1)
+            for (int i = lane; i < piece * G::row / 4; i += 32) {
+              reinterpret_cast<uint32_t*>(ring + slot * G::stage + q * piece * G::row)[i] = 0x88888888u;
+              reinterpret_cast<uint32_t*>(ring + slot * G::stage + G::half + q * piece * G::row)[i] = 0x88888888u;
+            }
+        fence_proxy_async_smem();                                        // the slot's next copy comes behind these stores
+        __syncwarp();
+      }
+        // scores: column tile j = (kk, t) holds in fragment column 2 c' + e the key 16 kk + 4 (2 t + e) + (c' ^ e): neighbouring lanes read neighbouring rows
+        float s[JT][4];
+#pragma unroll
+        for (int j = 0; j < JT; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+        for (int jb = 0; jb < JT; jb += 2) {
+#pragma unroll
+          for (int i0 = 0; i0 < G::words; i0 += (G::words < 4 ? G::words : 4)) {
+            constexpr int NW = G::words < 4 ? G::words : 4;
+            uint32_t w[2][NW];
+            I4Scale sc[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+              const int key = 16 * ((jb + j) >> 1) + 4 * (2 * (j & 1) + (n & 1)) + ((n >> 1) ^ (n & 1));
+              const uint8_t* src = kt + key * G::row + c * (G::row / 4) + 4 * i0;
+              if constexpr (NW == 2) { const uint2 x = *reinterpret_cast<const uint2*>(src); w[j][0] = x.x; w[j][1] = x.y; }
+              else { const uint4 x = *reinterpret_cast<const uint4*>(src); w[j][0] = x.x; w[j][1] = x.y; w[j][2] = x.z; w[j][3] = x.w; }
+              sc[j] = i4_scale(kt[G::codes + key * G::srow + (D == 64 ? c >> 1 : D == 128 ? c : 2 * c + i0 / 4)] * 0x00100010u);
+            }
+#pragma unroll
+            for (int i = 0; i < NW; i++) {
+              uint32_t qe[4], qo[4];
+              if constexpr (G::q_regs) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) { qe[r] = qa[2 * i][r]; qo[r] = qa[2 * i + 1][r]; }
+              } else {
+                const uint4 x = sq[(2 * (i0 + i)) * 32 + lane], y = sq[(2 * (i0 + i) + 1) * 32 + lane];
+                qe[0] = x.x; qe[1] = x.y; qe[2] = x.z; qe[3] = x.w;
+                qo[0] = y.x; qo[1] = y.y; qo[2] = y.z; qo[3] = y.w;
+              }
+#pragma unroll
+              for (int j = 0; j < 2; j++) mma_16816(s[jb + j], qe, i4_lower(w[j][i], sc[j]), i4_upper(w[j][i], sc[j]));
+#pragma unroll
+              for (int j = 0; j < 2; j++) mma_16816(s[jb + j], qo, i4_lower(w[j][i] >> 8, sc[j]), i4_upper(w[j][i] >> 8, sc[j]));
+            }
+          }
+        }
+        const int key0 = tile * G::keys;
+        if (key0 + G::keys - 1 > base_limit || (a.window > 0 && key0 <= max_limit - a.window)) {
+          const int low0 = a.window > 0 ? lim0 - a.window : -1, low1 = a.window > 0 ? lim1 - a.window : -1;
+#pragma unroll
+          for (int j = 0; j < JT; j++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const int key = key0 + 16 * (j >> 1) + 4 * (2 * (j & 1) + e) + (c ^ e);
+              if (key > lim0 || key <= low0) s[j][e] = -INFINITY;
+              if (key > lim1 || key <= low1) s[j][2 + e] = -INFINITY;
+            }
+        }
+        float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < JT; j++) {
+          x0 = fmaxf(x0, fmaxf(s[j][0], s[j][1]));
+          x1 = fmaxf(x1, fmaxf(s[j][2], s[j][3]));
+        }
+        x0 *= scale; x1 *= scale;
+        // the reference maximum moves only when a score exceeds it by more than 2^8 (or is the first): rare, so that the rows' lanes compare notes only then
+        if (__any_sync(0xffffffffu, x0 > m0 + 8.f || x1 > m1 + 8.f || (m0 == -INFINITY && x0 > m0) || (m1 == -INFINITY && x1 > m1))) {
+#pragma unroll
+          for (int d = 1; d < 4; d <<= 1) {
+            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+          }
+          const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+          const float f0 = n0 == -INFINITY ? 1.f : exp2f(m0 - n0), f1 = n1 == -INFINITY ? 1.f : exp2f(m1 - n1);
+          m0 = n0; m1 = n1;
+          l[0] *= f0; l[1] *= f0; l[2] *= f1; l[3] *= f1;
+#pragma unroll
+          for (int i = 0; i < G::nt; i++) { o[i][0] *= f0; o[i][1] *= f0; o[i][2] *= f1; o[i][3] *= f1; }
+        }
+        const float z0 = m0 == -INFINITY ? 0.f : -m0, z1 = m1 == -INFINITY ? 0.f : -m1;
+#pragma unroll
+        for (int kk = 0; kk < G::keys / 16; kk++) {
+          uint32_t pr[4];
+#pragma unroll
+          for (int t = 0; t < 2; t++) {
+            const float (&v)[4] = s[2 * kk + t];
+            pr[2 * t] = pack_bf16x2(exp2f(fmaf(v[0], scale, z0)), exp2f(fmaf(v[1], scale, z0)));
+            pr[2 * t + 1] = pack_bf16x2(exp2f(fmaf(v[2], scale, z1)), exp2f(fmaf(v[3], scale, z1)));
+          }
+          mma_16816(l, pr, 0x3F803F80u, 0x3F803F80u);                    // the sum of the probabilities as they are rounded
+          // values: this lane's four keys of the step, an eighth of each row
+          uint32_t w[4][G::vwords], sb[4];
+#pragma unroll
+          for (int x = 0; x < 4; x++) {
+            const int key = 16 * kk + 4 * x + (c ^ (x & 1));
+            const uint8_t* src = vt + key * G::row + n * (G::row / 8);
+            if constexpr (D == 64) w[x][0] = *reinterpret_cast<const uint32_t*>(src);
+            else if constexpr (D == 128) { const uint2 y = *reinterpret_cast<const uint2*>(src); w[x][0] = y.x; w[x][1] = y.y; }
+            else { const uint4 y = *reinterpret_cast<const uint4*>(src); w[x][0] = y.x; w[x][1] = y.y; w[x][2] = y.z; w[x][3] = y.w; }
+            sb[x] = vt[G::codes + key * G::srow + (D == 64 ? n >> 2 : D == 128 ? n >> 1 : n)];
+          }
+          const I4Scale sa = i4_scale(sb[0] * 16 + sb[1] * 0x100000u), sz = i4_scale(sb[2] * 16 + sb[3] * 0x100000u);
+#pragma unroll
+          for (int i = 0; i < G::vwords; i++) {
+            // a word's low half: even dims 0 2 4 6, high half: odd dims; two keys side by side
+            const uint32_t al = __byte_perm(w[0][i], w[1][i], 0x5410), ah = __byte_perm(w[0][i], w[1][i], 0x7632);
+            const uint32_t bl = __byte_perm(w[2][i], w[3][i], 0x5410), bh = __byte_perm(w[2][i], w[3][i], 0x7632);
+            mma_16816(o[8 * i + 0], pr, i4_lower(al, sa), i4_lower(bl, sz));
+            mma_16816(o[8 * i + 1], pr, i4_lower(ah, sa), i4_lower(bh, sz));
+            mma_16816(o[8 * i + 2], pr, i4_upper(al, sa), i4_upper(bl, sz));
+            mma_16816(o[8 * i + 3], pr, i4_upper(ah, sa), i4_upper(bh, sz));
+            mma_16816(o[8 * i + 4], pr, i4_lower(al >> 8, sa), i4_lower(bl >> 8, sz));
+            mma_16816(o[8 * i + 5], pr, i4_lower(ah >> 8, sa), i4_lower(bh >> 8, sz));
+            mma_16816(o[8 * i + 6], pr, i4_upper(al >> 8, sa), i4_upper(bl >> 8, sz));
+            mma_16816(o[8 * i + 7], pr, i4_upper(ah >> 8, sa), i4_upper(bh >> 8, sz));
+          }
+        }
+        __syncwarp();                                                    // every lane has read the slot
+      if (tile + ST < p.t_end) fetch(p, tile + ST, slot, id);
+      id = page_of(p, tile + ST + 1);
+      if (++slot == ST) { slot = 0; phase ^= 1; }
+    }
+
+    // what follows this piece, and its first copies
+    const bool whole = p.units == p.s.per_tile, head = p.unit == 0;
+    if (head && lane == 0) {                                             // the row tile's entry for the join: rows, first share with a piece of it, pieces
+      const int pieces = (int)((u0 + (min((long long)share, total.x - u0) - left) + p.s.per_tile - 1) / share) - mine + 1;
+      a.cuts[1 + p.index] = make_int4(tok0, max(0, n_tok * gh) | gh << 8 | pieces << 16, head0, mine);
+    }
+    left -= p.units;
+    if (left > 0) {
+      i4_next<G::keys>(a, sh, p, left);
+#pragma unroll 1
+      for (int i = 0; i < ST; i++)
+        if (p.t_begin + i < p.t_end) fetch(p, p.t_begin + i, slot + i < ST ? slot + i : slot + i - ST, page_of(p, p.t_begin + i));
+    }
+
+    const float inv0 = l[0] == 0.f ? 0.f : 16777216.f / l[0], inv1 = l[2] == 0.f ? 0.f : 16777216.f / l[2];       // a NaN stays one
+    const long long row0 = (long long)(tok0 + t0) * a.Hq + head0 + h0, row1 = (long long)(tok0 + t1) * a.Hq + head0 + h1;
+    const long long at = ((long long)mine * 2 + (head ? 1 : 0)) * 16;    // a row tile's first piece: the share's second place
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+      for (int i = 0; i < G::nt / 4; i++) {                              // dims (2 c + e) D/8 + 4 i ..
+        const int d = (2 * c + e) * (D / 8) + 4 * i;
+        const float4 x = make_float4(o[4 * i][e] * inv0, o[4 * i + 1][e] * inv0, o[4 * i + 2][e] * inv0, o[4 * i + 3][e] * inv0);
+        const float4 y = make_float4(o[4 * i][2 + e] * inv1, o[4 * i + 1][2 + e] * inv1, o[4 * i + 2][2 + e] * inv1, o[4 * i + 3][2 + e] * inv1);
+        if (whole) {
+          if (ok0) *reinterpret_cast<uint2*>(a.out + row0 * D + d) = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
+          if (ok1) *reinterpret_cast<uint2*>(a.out + row1 * D + d) = make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
+        } else {
+          if (ok0) *reinterpret_cast<float4*>(a.part + (at + n) * D + d) = x;
+          if (ok1) *reinterpret_cast<float4*>(a.part + (at + n + 8) * D + d) = y;
+        }
+      }
+    if (!whole && c == 0) {
+      if (ok0) a.lse2[at + n] = l[0] == 0.f ? -INFINITY : m0 + log2f(l[0]);
+      if (ok1) a.lse2[at + n + 8] = l[2] == 0.f ? -INFINITY : m1 + log2f(l[2]);
+    }
+    if (left == 0) break;
+  }
+}
+
+// Joins the pieces of row tile x where cuts run through it:  out = sum_p 2^(lse_p - m) part_p / sum_p 2^(lse_p - m).  The first piece sits in its share's second
+// place, the others' in their first.  Groups of D / 4 lanes
+// take a row each (kSplit false), or the groups of a CTA share the pieces of row y.
+constexpr int i4_join_threads(bool split) { return split ? 512 : 128; }
+template <int D, bool kSplit>
+__global__ void __launch_bounds__(i4_join_threads(kSplit)) gqa_int4_join_kernel(const I4Args a) {
+  pdl_wait(); pdl_trigger();
+  constexpr int Q = D / 4, GR = i4_join_threads(kSplit) / Q;             // quads of a row; groups
+  __shared__ float4 s_acc[kSplit ? GR : 1][Q];
+  __shared__ float s_sum[GR], s_max[GR];
+  const int4 cut = a.cuts[1 + blockIdx.x];
+  if ((int)blockIdx.x >= a.cuts[0].x) return;
+  const int rows = cut.y & 255, gh = cut.y >> 8 & 255, pieces = cut.y >> 16, first = cut.w;
+  if (pieces <= 1) return;
+  const int grp = threadIdx.x / Q, f = threadIdx.x % Q;
+  const int r = kSplit ? blockIdx.y : blockIdx.y * GR + grp;
+  if (r >= rows) return;                                                 // (kSplit: the whole CTA)
+  constexpr int kBatch = 8, step = kSplit ? GR : 1;                      // loads in flight; pieces between a group's
+  const int i0 = kSplit ? grp : 0;
+  auto place = [&](int i) { return ((long long)(first + i) * 2 + (i == 0)) * 16 + r; };
+  float m = -INFINITY, sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int b = i0; b < pieces; b += kBatch * step) {
+    float lse[kBatch];
+    float4 y[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; j++) {
+      const int i = b + j * step;
+      lse[j] = i < pieces ? a.lse2[place(i)] : -INFINITY;
+      y[j] = i < pieces ? *reinterpret_cast<const float4*>(a.part + place(i) * D + 4 * f) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < kBatch; j++) top = fmaxf(top, lse[j]);
+    const float old = m == -INFINITY ? 0.f : exp2f(m - top);
+    sum *= old; acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
+    m = top;
+#pragma unroll
+    for (int j = 0; j < kBatch; j++) {
+      const float wt = lse[j] == -INFINITY ? 0.f : m == -INFINITY ? lse[j] : exp2f(lse[j] - m);       // scores that are no numbers stay visible
+      sum += wt;
+      acc.x += wt * y[j].x; acc.y += wt * y[j].y; acc.z += wt * y[j].z; acc.w += wt * y[j].w;
+    }
+  }
+  if (kSplit) {
+    s_acc[grp][f] = acc;
+    if (f == 0) { s_sum[grp] = sum; s_max[grp] = m; }
     __syncthreads();
-    return;
-  }
-  float4* so = reinterpret_cast<float4*>(smem);                          // [W][16][D / 4], a row's quads swizzled within groups of eight
-  auto place = [](int row, int f) { return f ^ (((f >> 3) & 3) + 4 * (row & 1)); };
-#pragma unroll
-  for (int e = 0; e < 2; e++)
-#pragma unroll
-    for (int i = 0; i < G::nt / 4; i++) {                                // dims (2 c + e) D/8 + 4 i ..
-      const int f = (2 * c + e) * (G::nt / 4) + i;
-      so[(warp * 16 + r0) * (D / 4) + place(r0, f)] = make_float4(o[4 * i][e], o[4 * i + 1][e], o[4 * i + 2][e], o[4 * i + 3][e]);
-      so[(warp * 16 + r1) * (D / 4) + place(r1, f)] = make_float4(o[4 * i][2 + e], o[4 * i + 1][2 + e], o[4 * i + 2][2 + e], o[4 * i + 3][2 + e]);
-    }
-  if (c == 0) { s_m[warp][r0] = m0; s_m[warp][r1] = m1; s_l[warp][r0] = l0; s_l[warp][r1] = l1; }
-  __syncthreads();
-  for (int i = threadIdx.x; i < n_tok * gh * (D / 4); i += W * 32) {
-    const int r = i / (D / 4), f = i - r * (D / 4);
-    float m = -INFINITY, l = 0.f;
-    for (int w = 0; w < W; w++) m = fmaxf(m, s_m[w][r]);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = 0; w < W; w++) {
-      const float mw = s_m[w][r];
-      if (s_l[w][r] == 0.f) continue;                                    // saw no key
-      const float x = mw == -INFINITY ? 1.f : exp2f(mw - m);             // -inf: scores that are no numbers, which the sum shows
-      const float4 v = so[(w * 16 + r) * (D / 4) + place(r, f)];
-      l += x * s_l[w][r];
-      acc.x += x * v.x; acc.y += x * v.y; acc.z += x * v.z; acc.w += x * v.w;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;                          // a NaN stays one
-    const long long row = (long long)(tok0 + r / gh) * a.Hq + hkv * a.g + head0 + r % gh;
-    if (a.splits == 1) {
-      *reinterpret_cast<uint2*>(a.out + row * D + 4 * f) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-    } else {
-      const long long at = (long long)split * a.T * a.Hq + row;
-      *reinterpret_cast<float4*>(a.part + at * D + 4 * f) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-      if (f == 0) a.lse2[at] = l == 0.f ? -INFINITY : m + log2f(l);
+    if (grp > 0) return;
+    float top = -INFINITY;
+    for (int g = 0; g < GR; g++) top = fmaxf(top, s_max[g]);
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    sum = 0.f;
+    for (int g = 0; g < GR; g++) {
+      if (s_sum[g] == 0.f) continue;                                     // saw no key
+      const float wt = s_max[g] == -INFINITY ? 1.f : exp2f(s_max[g] - top);
+      const float4 z = s_acc[g][f];
+      sum += wt * s_sum[g];
+      acc.x += wt * z.x; acc.y += wt * z.y; acc.z += wt * z.z; acc.w += wt * z.w;
     }
   }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const long long row = (long long)(cut.x + r / gh) * a.Hq + cut.z + r % gh;
+  *reinterpret_cast<uint2*>(a.out + row * D + 4 * f) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
 }
 
 }  // namespace ne
@@ -324,41 +563,50 @@ __global__ void __launch_bounds__(W * 32, 1) gqa_int4_kernel(const I4Args a) {
 using namespace ne;
 
 namespace {
-template <int D, int W, int ST> int launch_i4(const I4Args& a, int tiles, cudaStream_t st) {
-  constexpr int ring = W * ST * I4Geo<D>::stage, join = W * 16 * D * 4, smem = ring > join ? ring : join;
-  static_assert(smem <= 225 * 1024, "shared memory of a CTA");
+template <int D, bool kPlain> cudaError_t launch_i4_main(const I4Args& a, cudaStream_t st) {
   static bool configured[64] = {};                                       // per device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return (int)e;
+  if (e != cudaSuccess) return e;
   if (dev >= 64 || !configured[dev]) {
-    e = cudaFuncSetAttribute(gqa_int4_kernel<D, W, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return (int)e;
+    e = cudaFuncSetAttribute(gqa_int4_kernel<D, kPlain>, cudaFuncAttributeMaxDynamicSharedMemorySize, I4Geo<D>::smem);
+    if (e != cudaSuccess) return e;
     if (dev < 64) configured[dev] = true;
   }
-  return (int)launch_pdl(gqa_int4_kernel<D, W, ST>, dim3((unsigned)tiles, (unsigned)(a.Hkv * a.head_tiles), (unsigned)a.splits), dim3(W * 32), smem, st, a);
+  return launch_pdl(gqa_int4_kernel<D, kPlain>, dim3((unsigned)(a.shares / kI4Warps)), dim3(kI4Threads), I4Geo<D>::smem, st, a);
+}
+template <int D> int launch_i4(const I4Args& a, int tiles, cudaStream_t st) {
+  const cudaError_t e = a.block_size % I4Geo<D>::keys == 0 ? launch_i4_main<D, true>(a, st) : launch_i4_main<D, false>(a, st);
+  if (e != cudaSuccess) return (int)e;
+  // pieces of a row tile: where they are many, a CTA per row shares them (us of both forms, 1184 shares: 8 row tiles 2.6 / 8.2, 120 row tiles 7.8 / 2.9)
+  if (a.shares > 16 * tiles) return (int)launch_pdl(gqa_int4_join_kernel<D, true>, dim3((unsigned)tiles, 16), dim3(i4_join_threads(true)), 0, st, a);
+  return (int)launch_pdl(gqa_int4_join_kernel<D, false>, dim3((unsigned)tiles, D / 32), dim3(i4_join_threads(false)), 0, st, a);
 }
 }  // namespace
 
-// q bf16 [T, Hq, D] with rows q_ld elements apart (8-byte aligned); k / v uint8 [num_blocks, Hkv, block_size (D/2 + D/32)].  tiles: an upper bound of the sum over
-// sequences of ceil(q_len / tq), tq = max(1, 16 / g).  splits > 1: part / lse2 as ne_attn_merge takes them.
+// Shares of the work that an SM's CTAs hold for heads of D (0: not built for them)
+extern "C" int ne_gqa_int4_shares(int D) { return kI4Warps * (D == 64 ? I4Geo<64>::ctas : D == 128 ? I4Geo<128>::ctas : D == 256 ? I4Geo<256>::ctas : 0); }
+
+// q bf16 [T, Hq, D] with rows q_ld elements apart (8-byte aligned); k / v uint8 [num_blocks, Hkv, block_size (D/2 + D/32)].  shares: of the work, a multiple of 4, each with
+// two places of 16 rows in part fp32 [shares, 2, 16, D] and lse2 fp32 [shares, 2, 16].  tiles: an upper bound of the row tiles, the sum over sequences of
+// ceil(q_len / tq) Hkv ceil(g / 16), tq = max(1, 16 / g); cuts int32 [1 + tiles, 4].
 extern "C" int ne_gqa_int4(const void* q, long long q_ld, const void* k, const void* v, int num_blocks, int block_size, const int* block_tables, long long bt_ld, int bt_width,
-                           const int* cu_seqlens_q, const int* context_lens, int num_seqs, int T, int Hq, int Hkv, int D, int tiles, int splits, int window, float scale,
-                           void* out, float* part, float* lse2, cudaStream_t st) {
+                           const int* cu_seqlens_q, const int* context_lens, int num_seqs, int T, int Hq, int Hkv, int D, int shares, int tiles, int window, float scale,
+                           void* out, float* part, float* lse2, void* cuts, cudaStream_t st) {
   if (T <= 0 || num_seqs <= 0) return 0;
-  if (Hkv < 1 || Hq < Hkv || Hq % Hkv || num_blocks < 1 || bt_width < 1 || tiles < 1 || splits < 1 || splits > 65535 || (splits > 1 && (!part || !lse2))) return 1001;
-  if (!(block_size == 16 || block_size == 32 || (block_size > 0 && block_size % kTileKeys == 0))) return 1002;
+  if (Hkv < 1 || Hq < Hkv || Hq % Hkv || num_blocks < 1 || bt_width < 1 || shares < kI4Warps || shares % kI4Warps || shares >= 32768 || tiles < 1 || !part || !lse2 || !cuts)
+    return 1001;
+  if (!(block_size == 16 || block_size == 32 || (block_size > 0 && block_size % 64 == 0))) return 1002;
   I4Args a{};
   a.q = (const __nv_bfloat16*)q; a.q_ld = q_ld; a.k = (const uint8_t*)k; a.v = (const uint8_t*)v; a.num_blocks = num_blocks; a.block_size = block_size;
   a.block_tables = block_tables; a.bt_ld = bt_ld; a.bt_width = bt_width; a.cu_seqlens_q = cu_seqlens_q; a.context_lens = context_lens; a.num_seqs = num_seqs;
-  a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.g = Hq / Hkv; a.tq = a.g >= 16 ? 1 : 16 / a.g; a.head_tiles = (a.g + 15) / 16; a.splits = splits;
+  a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.g = Hq / Hkv; a.tq = a.g >= 16 ? 1 : 16 / a.g; a.head_tiles = (a.g + 15) / 16; a.shares = shares;
   a.window = window > 0 ? window : 0; a.scale_log2 = scale * 1.4426950408889634f;
-  a.out = (__nv_bfloat16*)out; a.part = part; a.lse2 = lse2;
-  if ((long long)Hkv * a.head_tiles > 65535) return 1003;
+  a.out = (__nv_bfloat16*)out; a.part = part; a.lse2 = lse2; a.cuts = (int4*)cuts;
   switch (D) {
-    case 64: return launch_i4<64, 8, 4>(a, tiles, st);
-    case 128: return launch_i4<128, 8, 3>(a, tiles, st);
-    case 256: return launch_i4<256, 6, 2>(a, tiles, st);
+    case 64: return launch_i4<64>(a, tiles, st);
+    case 128: return launch_i4<128>(a, tiles, st);
+    case 256: return launch_i4<256>(a, tiles, st);
     default: return 1004;
   }
 }

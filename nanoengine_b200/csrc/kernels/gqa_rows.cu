@@ -4,9 +4,9 @@
 //   y = x / sqrt(mean x^2 + eps) w ;  pairs (i, i + D/2) of y turned by the angle of position[axis(i)]
 //   4 bits, groups of 32 dims:  s = amax / 7 to four significant bits,  c = clamp(rint(y / s), -7, 7) + 8
 //
-// Bound by HBM: a row is read once and written once (a key or value as D/2 + D/32 bytes).  One warp takes the heads of one token one after the other:
-// lane l holds the dims [l E, l E + E), E = D / 32, so that a row is one load per lane, its rotation partner sits in lane l ^ 16, a group of 32
-// dims in 32 / E neighbouring lanes, and the cosines and sines are fetched once for all heads.
+// Bound by HBM: a row is read once and written once (a key or value as D/2 + D/32 bytes).  A lane holds four dims of the lower half of a row and their
+// partners in the upper half, so that a rotation stays in the lane; D / 8 lanes share a row, a warp takes 256 / D heads of one token at a time.  Query rows
+// go in batches of four such steps, loaded before the first is used, under one fetch of cosines and sines.
 //
 // The key row that is cut to 4 bits is computed in 64 bits: its codes sit on borders, and a sum taken in another order would move some of them.  Value
 // rows are bf16, whose quotients are exact or far from a border in 32 bits.  Built without approximate functions.
@@ -15,6 +15,7 @@
 namespace ne {
 
 constexpr int kRowsWarps = 8;
+constexpr int kRowsBatch = 4;                         // steps of query rows in flight
 constexpr double kKv4Most = 7 * 1.875 * 32768;       // largest value of the format
 
 struct RowsArgs {
@@ -23,116 +24,136 @@ struct RowsArgs {
   const long long* positions; long long pos_ld; const float* rope; int max_pos;
   int axes, interleaved, sections[4];
   __nv_bfloat16* q_out; uint8_t* k_cache; uint8_t* v_cache; const long long* slots; long long cache_rows;
-  int T, Hq, Hkv, block_size, chunk;                  // chunk: heads of a warp
+  int T, Hq, Hkv, block_size, chunk;                  // chunk: steps of query rows a warp takes
 };
 
-template <int E> struct RowBits { uint32_t u[(E + 1) / 2]; };
-
-template <int E> __device__ __forceinline__ RowBits<E> load_bits(const __nv_bfloat16* p) {
-  RowBits<E> r;
-  if constexpr (E == 1) r.u[0] = *reinterpret_cast<const uint16_t*>(p);
-  else if constexpr (E == 2) r.u[0] = *reinterpret_cast<const uint32_t*>(p);
-  else if constexpr (E == 4) { const uint2 v = *reinterpret_cast<const uint2*>(p); r.u[0] = v.x; r.u[1] = v.y; }
-  else { const uint4 v = *reinterpret_cast<const uint4*>(p); r.u[0] = v.x; r.u[1] = v.y; r.u[2] = v.z; r.u[3] = v.w; }
-  return r;
+// a lane's dims of a row: [4 l, 4 l + 4) and their partners half a row further
+struct RowBits { uint2 lo, hi; };
+template <int L> __device__ __forceinline__ RowBits load_row(const __nv_bfloat16* row, int l) {
+  return {*reinterpret_cast<const uint2*>(row + 4 * l), *reinterpret_cast<const uint2*>(row + 4 * L + 4 * l)};
 }
-template <int E> __device__ __forceinline__ float bits_at(const RowBits<E>& r, int e) {
-  return __uint_as_float(e & 1 ? r.u[e >> 1] & 0xffff0000u : r.u[e >> 1] << 16);
-}
-template <int E> __device__ __forceinline__ void store_bf16(__nv_bfloat16* p, const float (&v)[E]) {
-  if constexpr (E == 1) *p = __float2bfloat16(v[0]);
-  else {
-    uint32_t u[E / 2];
+__device__ __forceinline__ void unpack_row(const RowBits& b, float (&x)[8]) {
+  const uint32_t u[4] = {b.lo.x, b.lo.y, b.hi.x, b.hi.y};
 #pragma unroll
-    for (int i = 0; i < E / 2; i++) u[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
-    if constexpr (E == 2) *reinterpret_cast<uint32_t*>(p) = u[0];
-    else if constexpr (E == 4) *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
-    else *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
-  }
+  for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(u[i] << 16); x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
+}
+template <int L> __device__ __forceinline__ void store_row(__nv_bfloat16* row, int l, const float (&x)[8]) {
+  *reinterpret_cast<uint2*>(row + 4 * l) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+  *reinterpret_cast<uint2*>(row + 4 * L + 4 * l) = make_uint2(pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
 }
 
-// norm and rotation of one row in R (float or double); all lanes of the warp
-template <int E, typename R> __device__ __forceinline__ void norm_and_turn(R (&x)[E], const __nv_bfloat16* w, double eps, float w_offset, const float (&cs)[E],
-                                                                           const float (&sn)[E], int lane) {
-  if (w) {
+// norm and rotation of one row in R (float or double), by its L lanes
+template <int L, typename R> __device__ __forceinline__ void norm_and_turn(R (&x)[8], const RowBits& w, bool norm, double eps, float w_offset, const float (&cs)[4],
+                                                                           const float (&sn)[4]) {
+  if (norm) {
     R ss = 0;
 #pragma unroll
-    for (int e = 0; e < E; e++) ss += x[e] * x[e];
+    for (int e = 0; e < 8; e++) ss += x[e] * x[e];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const R r = rsqrt(ss / (R)(32 * E) + (R)eps);
-    const RowBits<E> g = load_bits<E>(w + lane * E);
+    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const R r = rsqrt(ss / (R)(8 * L) + (R)eps);
+    float g[8];
+    unpack_row(w, g);
 #pragma unroll
-    for (int e = 0; e < E; e++) x[e] = x[e] * r * ((R)bits_at(g, e) + (R)w_offset);
+    for (int e = 0; e < 8; e++) x[e] = x[e] * r * ((R)g[e] + (R)w_offset);
   }
-  const bool low = lane < 16;
 #pragma unroll
-  for (int e = 0; e < E; e++) {
-    const R other = __shfl_xor_sync(0xffffffffu, x[e], 16);
-    x[e] = low ? x[e] * (R)cs[e] - other * (R)sn[e] : x[e] * (R)cs[e] + other * (R)sn[e];
+  for (int e = 0; e < 4; e++) {
+    const R a = x[e], b = x[4 + e];
+    x[e] = a * (R)cs[e] - b * (R)sn[e];
+    x[4 + e] = b * (R)cs[e] + a * (R)sn[e];
   }
 }
 
-// Scale byte of a group whose largest magnitude is amax, and the scale itself: amax / 7 to four significant bits, ties to even.
-__device__ __forceinline__ int kv4_scale_of(double amax, double* s) {
-  const unsigned long long u = (unsigned long long)__double_as_longlong(amax / 7.0);
-  const long long r = (long long)((u + ((1ull << 48) - 1) + ((u >> 49) & 1)) >> 49) - (1023 - 16) * 8;
-  const int b = (int)(r < 0 ? 0 : r > 255 ? 255 : r);
-  *s = __longlong_as_double((long long)(b + (1023 - 16) * 8) << 49);
+// Scale byte of a group whose largest magnitude is amax: the nearest scale to amax / 7, ties to the even byte, and the scale itself.  A first guess in 32 bits is
+// corrected by comparing amax with seven times the midpoints, products of few bits that are exact.
+__device__ __forceinline__ float kv4_scale_value(int b) { return __uint_as_float((uint32_t)(b + (127 - 16) * 8) << 20); }
+template <typename R> __device__ __forceinline__ int kv4_scale_of(R amax, float* s) {
+  const uint32_t u = __float_as_uint(__fdiv_rn((float)amax, 7.f));
+  int b = (int)((u + (1u << 19)) >> 20) - (127 - 16) * 8;
+  b = min(max(b, 0), 255);
+  const float lo = kv4_scale_value(max(b - 1, 0)), at = kv4_scale_value(b), hi = kv4_scale_value(min(b + 1, 255));
+  const R up = (R)3.5 * ((R)at + (R)hi), down = (R)3.5 * ((R)lo + (R)at);
+  if (b < 255 && (amax > up || (amax == up && (b & 1)))) b++;
+  else if (b > 0 && (amax < down || (amax == down && (b & 1)))) b--;
+  *s = kv4_scale_value(b);
   return b;
 }
-__device__ __forceinline__ int kv4_scale_of(float amax, float* s) {
-  const uint32_t u = __float_as_uint(__fdiv_rn(amax, 7.f));
-  const int r = (int)((u + ((1u << 19) - 1) + ((u >> 20) & 1)) >> 20) - (127 - 16) * 8;
-  const int b = r < 0 ? 0 : r > 255 ? 255 : r;
-  *s = __uint_as_float((uint32_t)(b + (127 - 16) * 8) << 20);
-  return b;
+// The nearest multiple of s, ties to even, from -7 to 7: by a product with the reciprocal, corrected with the exact remainder.
+__device__ __forceinline__ int kv4_code(float x, float s, float inv) {
+  const float t = fmaf(x, inv, 12582912.f);
+  int q = __float_as_int(t) - 0x4B400000;
+  const float r = fmaf(-(t - 12582912.f), s, x), h = 0.5f * s;
+  if (r > h || (r == h && (q & 1))) q++;
+  else if (r < -h || (r == -h && (q & 1))) q--;
+  return min(max(q, -7), 7);
 }
-__device__ __forceinline__ int kv4_code(double x, double s) { return (int)rint(x / s); }
-__device__ __forceinline__ int kv4_code(float x, float s) { return (int)rintf(__fdiv_rn(x, s)); }
+__device__ __forceinline__ int kv4_code(double x, float sf, float inv) {
+  const double s = sf, t = fma(x, (double)inv, 6755399441055744.0);
+  int q = __double2loint(t);
+  const double r = fma(-(t - 6755399441055744.0), s, x), h = 0.5 * s;
+  if (r > h || (r == h && (q & 1))) q++;
+  else if (r < -h || (r == -h && (q & 1))) q--;
+  return min(max(q, -7), 7);
+}
 
-// one row [32 E] of a head to its place in a 4-bit page; all lanes of the warp
-template <int E, typename R> __device__ __forceinline__ void store_kv4(uint8_t* page, int tok, int block_size, R (&x)[E], int lane) {
-  R amax = 0;
+// one row [8 L] of a head to its place in a 4-bit page, by its L lanes (all lanes of the warp call; those without a row pass store = false)
+template <int L, typename R> __device__ __forceinline__ void store_kv4(uint8_t* page, int tok, int block_size, R (&x)[8], int l, bool store) {
+  constexpr int D = 8 * L;
+  R m0 = 0, m1 = 0;
 #pragma unroll
-  for (int e = 0; e < E; e++) {
+  for (int e = 0; e < 8; e++) {
     x[e] = x[e] != x[e] ? (R)0 : x[e] > (R)kKv4Most ? (R)kKv4Most : x[e] < -(R)kKv4Most ? -(R)kKv4Most : x[e];
     const R m = x[e] < 0 ? -x[e] : x[e];
-    amax = m > amax ? m : amax;
+    if (e < 4) m0 = m > m0 ? m : m0; else m1 = m > m1 ? m : m1;
   }
+  if (L == 4) m0 = m1 = m0 > m1 ? m0 : m1;                               // one group of 32: both halves
 #pragma unroll
-  for (int o = 16 / E; o > 0; o >>= 1) { const R m = __shfl_xor_sync(0xffffffffu, amax, o); amax = m > amax ? m : amax; }
-  R s;
-  const int b = kv4_scale_of(amax, &s);
-  uint32_t w = 0;
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    const int c = min(max(kv4_code(x[e], s), -7), 7) + 8, d = (lane * E + e) & 7;
-    w |= (uint32_t)c << (4 * ((d >> 1) + 4 * (d & 1)));
+  for (int o = L == 4 ? 2 : 4; o > 0; o >>= 1) {
+    const R a = __shfl_xor_sync(0xffffffffu, m0, o), b = L == 4 ? a : __shfl_xor_sync(0xffffffffu, m1, o);
+    m0 = a > m0 ? a : m0;
+    m1 = b > m1 ? b : m1;
   }
+  float s0, s1;
+  const int b0 = kv4_scale_of(m0, &s0), b1 = L == 4 ? b0 : kv4_scale_of(m1, &s1);
+  if (L == 4) s1 = s0;
+  const float i0 = __fdiv_rn(1.f, s0), i1 = L == 4 ? i0 : __fdiv_rn(1.f, s1);
+  int c[8];
 #pragma unroll
-  for (int o = 4 / E; o > 0; o >>= 1) w |= __shfl_xor_sync(0xffffffffu, w, o);
-  constexpr int D = 32 * E;
-  if ((lane * E) % 8 == 0) *reinterpret_cast<uint32_t*>(page + tok * (D / 2) + lane * E / 2) = w;
-  if ((lane * E) % 32 == 0) page[block_size * (D / 2) + tok * (D / 32) + lane * E / 32] = (uint8_t)b;
+  for (int e = 0; e < 8; e++) c[e] = kv4_code(x[e], e < 4 ? s0 : s1, e < 4 ? i0 : i1) + 8;
+  // four dims of a word of eight: even places in one byte of the low half, odd ones in one of the high half
+  const int sh = 8 * (l & 1);
+  const uint32_t w0 = (uint32_t)(c[0] | c[2] << 4) << sh | (uint32_t)(c[1] | c[3] << 4) << (16 + sh);
+  const uint32_t w1 = (uint32_t)(c[4] | c[6] << 4) << sh | (uint32_t)(c[5] | c[7] << 4) << (16 + sh);
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, l & 1 ? w0 : w1, 1);
+  if (!store) return;
+  // even lanes write the word of the lower half, odd lanes that of the upper half
+  *reinterpret_cast<uint32_t*>(page + tok * (D / 2) + (l & 1 ? D / 4 : 0) + (l >> 1) * 4) = (l & 1 ? w1 : w0) | other;
+  if (l % 8 < (L == 4 ? 1 : 2)) page[block_size * (D / 2) + tok * (D / 32) + (l & 1 ? D / 64 : 0) + (l >> 3)] = (uint8_t)(l & 1 ? b1 : b0);
 }
 
-template <int E, bool kInt4>
+__device__ __forceinline__ void split_slot(long long slot, int block_size, long long& page, int& tok) {
+  if (slot < (1ll << 31)) { page = (unsigned)slot / (unsigned)block_size; tok = (int)((unsigned)slot % (unsigned)block_size); }
+  else { page = slot / block_size; tok = (int)(slot % block_size); }
+}
+
+// A warp takes `chunk` steps of a token's query heads, or one step of its key heads, or of its value heads; a step is the heads of 32 / L rows.
+template <int L, bool kInt4>
 __global__ void __launch_bounds__(kRowsWarps * 32) gqa_rows_kernel(const RowsArgs a) {
   pdl_wait(); pdl_trigger();
-  constexpr int D = 32 * E;
-  const int heads = a.Hq + 2 * a.Hkv, lane = threadIdx.x & 31;
-  const int chunks = (heads + a.chunk - 1) / a.chunk;
+  constexpr int D = 8 * L, R = 32 / L;
+  const int lane = threadIdx.x & 31, l = lane % L, sub = lane / L;
+  const int q_steps = (a.Hq + R - 1) / R, kv_steps = (a.Hkv + R - 1) / R, q_warps = (q_steps + a.chunk - 1) / a.chunk, per_token = q_warps + 2 * kv_steps;
   const long long w = (long long)blockIdx.x * kRowsWarps + (threadIdx.x >> 5);
-  if (w >= (long long)a.T * chunks) return;
-  const int t = (int)(w / chunks), h0 = (int)(w - (long long)t * chunks) * a.chunk, h1 = min(h0 + a.chunk, heads);
-  const __nv_bfloat16* src = a.qkv + (long long)t * a.ld + lane * E;
-  RowBits<E> next = load_bits<E>(src + (long long)h0 * D);
-  float cs[E], sn[E];
-  if (h0 < a.Hq + a.Hkv) {
+  if (w >= (long long)a.T * per_token) return;
+  const int t = (int)(w / per_token), part = (int)(w - (long long)t * per_token);
+  const __nv_bfloat16* src = a.qkv + (long long)t * a.ld;
+  const bool is_q = part < q_warps, is_v = part >= q_warps + kv_steps;
+  float cs[4], sn[4];
+  auto angles = [&] {
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-      const int i = (lane & 15) * E + e;                                     // angle of the pair (i, i + D/2)
+    for (int e = 0; e < 4; e++) {
+      const int i = 4 * l + e;                                               // angle of the pair (i, i + D/2)
       int ax = 0;
       if (a.axes > 1) {
         if (a.interleaved) {
@@ -148,65 +169,91 @@ __global__ void __launch_bounds__(kRowsWarps * 32) gqa_rows_kernel(const RowsArg
       cs[e] = a.rope[pos * D + i];
       sn[e] = a.rope[pos * D + D / 2 + i];
     }
-  }
-  const long long slot = h1 > a.Hq ? a.slots[t] : -1;
-  const bool store = slot >= 0 && slot < a.cache_rows && NE_INDEX_OK(slot, BK_CACHE_ROWS, 30, __LINE__);
-  long long page = 0; int tok = 0;
-  if (kInt4 && store) {
-    if (slot < (1ll << 31)) { page = (unsigned)slot / (unsigned)a.block_size; tok = (int)((unsigned)slot % (unsigned)a.block_size); }
-    else { page = slot / a.block_size; tok = (int)(slot % a.block_size); }
-  }
-  for (int h = h0; h < h1; h++) {
-    const RowBits<E> now = next;
-    if (h + 1 < h1) next = load_bits<E>(src + (long long)(h + 1) * D);
-    const bool is_q = h < a.Hq, is_k = !is_q && h < a.Hq + a.Hkv;
-    if (!is_q && !store) break;                                              // keys and values come last: nothing more to do
-    float x[E];
+  };
+  if (is_q) {
+    RowBits next[kRowsBatch];
+    const int s0 = part * a.chunk, s1 = min(s0 + a.chunk, q_steps);
 #pragma unroll
-    for (int e = 0; e < E; e++) x[e] = bits_at(now, e);
-    if (is_q) {
-      norm_and_turn<E, float>(x, a.qw, a.eps, a.w_offset, cs, sn, lane);
-      store_bf16<E>(a.q_out + ((long long)t * a.Hq + h) * D + lane * E, x);
-      continue;
+    for (int i = 0; i < kRowsBatch; i++) {
+      const int h = (s0 + i) * R + sub;
+      if (s0 + i < s1 && h < a.Hq) next[i] = load_row<L>(src + (long long)h * D, l); else next[i] = {make_uint2(0, 0), make_uint2(0, 0)};
     }
-    const int kh = is_k ? h - a.Hq : h - a.Hq - a.Hkv;
-    uint8_t* cache = is_k ? a.k_cache : a.v_cache;
-    if constexpr (kInt4) {
-      uint8_t* dst = cache + (page * a.Hkv + kh) * ((long long)a.block_size * (D / 2 + D / 32));
-      if (is_k) {
-        double y[E];
+    RowBits g = {make_uint2(0, 0), make_uint2(0, 0)};
+    if (a.qw) g = load_row<L>(a.qw, l);
+    angles();
+    for (int s = s0; s < s1; s += kRowsBatch) {
+      RowBits now[kRowsBatch];
 #pragma unroll
-        for (int e = 0; e < E; e++) y[e] = x[e];
-        norm_and_turn<E, double>(y, a.kw, a.eps, a.w_offset, cs, sn, lane);
-        store_kv4<E, double>(dst, tok, a.block_size, y, lane);
-      } else {
-        store_kv4<E, float>(dst, tok, a.block_size, x, lane);
+      for (int i = 0; i < kRowsBatch; i++) {
+        now[i] = next[i];
+        const int h = (s + kRowsBatch + i) * R + sub;
+        if (s + kRowsBatch + i < s1 && h < a.Hq) next[i] = load_row<L>(src + (long long)h * D, l);
       }
-    } else {
-      if (is_k) norm_and_turn<E, float>(x, a.kw, a.eps, a.w_offset, cs, sn, lane);
-      store_bf16<E>(reinterpret_cast<__nv_bfloat16*>(cache) + (slot * a.Hkv + kh) * D + lane * E, x);
+#pragma unroll
+      for (int i = 0; i < kRowsBatch; i++) {
+        if (s + i >= s1) break;
+        float x[8];
+        unpack_row(now[i], x);
+        norm_and_turn<L, float>(x, g, a.qw != nullptr, a.eps, a.w_offset, cs, sn);
+        const int h = (s + i) * R + sub;
+        if (h < a.Hq) store_row<L>(a.q_out + ((long long)t * a.Hq + h) * D, l, x);
+      }
     }
+    return;
+  }
+  const long long slot = a.slots[t];
+  if (slot < 0 || slot >= a.cache_rows || !NE_INDEX_OK(slot, BK_CACHE_ROWS, 30, __LINE__)) return;
+  const int h = (part - q_warps - (is_v ? kv_steps : 0)) * R + sub;
+  const bool live = h < a.Hkv;
+  RowBits bits = {make_uint2(0, 0), make_uint2(0, 0)}, g = bits;
+  if (live) bits = load_row<L>(src + (long long)(a.Hq + (is_v ? a.Hkv : 0) + h) * D, l);
+  if (!is_v) {
+    if (a.kw) g = load_row<L>(a.kw, l);
+    angles();
+  }
+  float x[8];
+  unpack_row(bits, x);
+  uint8_t* cache = is_v ? a.v_cache : a.k_cache;
+  if constexpr (kInt4) {
+    long long page; int tok;
+    split_slot(slot, a.block_size, page, tok);
+    uint8_t* dst = cache + (page * a.Hkv + (live ? h : 0)) * ((long long)a.block_size * (D / 2 + D / 32));
+    if (is_v) {
+      store_kv4<L, float>(dst, tok, a.block_size, x, l, live);
+    } else {
+      double y[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) y[e] = x[e];
+      norm_and_turn<L, double>(y, g, a.kw != nullptr, a.eps, a.w_offset, cs, sn);
+      store_kv4<L, double>(dst, tok, a.block_size, y, l, live);
+    }
+  } else {
+    if (!is_v) norm_and_turn<L, float>(x, g, a.kw != nullptr, a.eps, a.w_offset, cs, sn);
+    if (live) store_row<L>(reinterpret_cast<__nv_bfloat16*>(cache) + (slot * a.Hkv + h) * D, l, x);
   }
 }
 
-// Rows of k and v [T, Hkv, D] as they are into 4-bit pages: a warp per (token, head, key or value).
-template <int E>
+// Rows of k and v [T, Hkv, D] as they are into 4-bit pages: a warp per (token, step of heads, key or value).
+template <int L>
 __global__ void __launch_bounds__(kRowsWarps * 32) kv4_store_kernel(const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ v, long long k_ld, long long v_ld,
                                                                    uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache, const long long* __restrict__ slots,
                                                                    long long cache_rows, int T, int Hkv, int block_size) {
   pdl_wait(); pdl_trigger();
-  constexpr int D = 32 * E;
-  const int lane = threadIdx.x & 31;
+  constexpr int D = 8 * L, R = 32 / L;
+  const int lane = threadIdx.x & 31, l = lane % L, steps = (Hkv + R - 1) / R;
   const long long w = (long long)blockIdx.x * kRowsWarps + (threadIdx.x >> 5);
-  if (w >= (long long)T * 2 * Hkv) return;
-  const int t = (int)(w / (2 * Hkv)), r = (int)(w - (long long)t * 2 * Hkv), h = r >> 1;
+  if (w >= (long long)T * 2 * steps) return;
+  const int t = (int)(w / (2 * steps)), r = (int)(w - (long long)t * 2 * steps), h = (r >> 1) * R + lane / L;
   const long long slot = slots[t];
   if (slot < 0 || slot >= cache_rows || !NE_INDEX_OK(slot, BK_CACHE_ROWS, 30, __LINE__)) return;
-  const RowBits<E> bits = load_bits<E>((r & 1 ? v + (long long)t * v_ld : k + (long long)t * k_ld) + h * D + lane * E);
-  float x[E];
-#pragma unroll
-  for (int e = 0; e < E; e++) x[e] = bits_at(bits, e);
-  store_kv4<E, float>((r & 1 ? v_cache : k_cache) + (slot / block_size * Hkv + h) * ((long long)block_size * (D / 2 + D / 32)), (int)(slot % block_size), block_size, x, lane);
+  const bool live = h < Hkv;
+  RowBits bits = {make_uint2(0, 0), make_uint2(0, 0)};
+  if (live) bits = load_row<L>((r & 1 ? v + (long long)t * v_ld : k + (long long)t * k_ld) + h * D, l);
+  float x[8];
+  unpack_row(bits, x);
+  long long page; int tok;
+  split_slot(slot, block_size, page, tok);
+  store_kv4<L, float>((r & 1 ? v_cache : k_cache) + (page * Hkv + (live ? h : 0)) * ((long long)block_size * (D / 2 + D / 32)), tok, block_size, x, l, live);
 }
 
 // 4-bit rows as bf16 [T, Hkv, D]: a thread per word of 8 dims of a key and a value row.  Slots outside the cache give zeros.
@@ -248,21 +295,32 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(const uint8_t* __restri
   }
   if (p * 64 >= n) return;
   const int words = D / 8;
-  for (int i = threadIdx.x; i < 64 * words; i += 256) {
-    const int r = i / words, j = i - r * words, key = p * 64 + r;
-    uint4 kv = make_uint4(0, 0, 0, 0), vv = kv;
-    if (key < n) {
-      const int id = tables[(long long)seq * bt_ld + key / block_size], tok = key % block_size;
-      if (id >= 0 && id < num_blocks && NE_INDEX_OK(id, BK_CACHE_PAGES, 30, __LINE__)) {
-        const long long base = ((long long)id * Hkv + h) * ((long long)block_size * (D / 2 + D / 32));
-        const long long code = base + tok * (D / 2) + 4 * j, scale = base + block_size * (D / 2) + tok * (D / 32) + j / 4;
-        kv = kv4_word(*reinterpret_cast<const uint32_t*>(k_cache + code), k_cache[scale]);
-        vv = kv4_word(*reinterpret_cast<const uint32_t*>(v_cache + code), v_cache[scale]);
+  constexpr int kFlight = 4;                                             // words of a thread in flight
+  for (int i0 = threadIdx.x; i0 < 64 * words; i0 += 256 * kFlight) {
+    uint32_t kw[kFlight], vw[kFlight], ks[kFlight], vs[kFlight];
+#pragma unroll
+    for (int u = 0; u < kFlight; u++) {
+      const int i = i0 + u * 256, r = i / words, j = i - r * words, key = p * 64 + r;
+      kw[u] = vw[u] = 0x88888888u;                                       // zeros
+      ks[u] = vs[u] = 0;
+      if (r < 64 && key < n) {
+        const int id = tables[(long long)seq * bt_ld + key / block_size], tok = key % block_size;
+        if (id >= 0 && id < num_blocks && NE_INDEX_OK(id, BK_CACHE_PAGES, 30, __LINE__)) {
+          const long long base = ((long long)id * Hkv + h) * ((long long)block_size * (D / 2 + D / 32));
+          const long long code = base + tok * (D / 2) + 4 * j, scale = base + block_size * (D / 2) + tok * (D / 32) + j / 4;
+          kw[u] = *reinterpret_cast<const uint32_t*>(k_cache + code); ks[u] = k_cache[scale];
+          vw[u] = *reinterpret_cast<const uint32_t*>(v_cache + code); vs[u] = v_cache[scale];
+        }
       }
     }
-    const long long dst = ((at * 64 + r) * Hkv + h) * D + 8 * j;
-    *reinterpret_cast<uint4*>(k_out + dst) = kv;
-    *reinterpret_cast<uint4*>(v_out + dst) = vv;
+#pragma unroll
+    for (int u = 0; u < kFlight; u++) {
+      const int i = i0 + u * 256, r = i / words, j = i - r * words;
+      if (r >= 64) break;
+      const long long dst = ((at * 64 + r) * Hkv + h) * D + 8 * j;
+      *reinterpret_cast<uint4*>(k_out + dst) = kv4_word(kw[u], ks[u]);
+      *reinterpret_cast<uint4*>(v_out + dst) = kv4_word(vw[u], vs[u]);
+    }
   }
 }
 
@@ -271,31 +329,35 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(const uint8_t* __restri
 using namespace ne;
 
 namespace {
-template <int E> cudaError_t launch_rows(const RowsArgs& a, bool int4, cudaStream_t st) {
-  const long long warps = (long long)a.T * ((a.Hq + 2 * a.Hkv + a.chunk - 1) / a.chunk);
+template <int L> int launch_rows(const RowsArgs& a, bool int4, cudaStream_t st) {
+  constexpr int R = 32 / L;
+  const int q_steps = (a.Hq + R - 1) / R, kv_steps = (a.Hkv + R - 1) / R;
+  const long long warps = (long long)a.T * ((q_steps + a.chunk - 1) / a.chunk + 2 * kv_steps);
   const dim3 grid((unsigned)((warps + kRowsWarps - 1) / kRowsWarps));
-  return int4 ? launch_pdl(gqa_rows_kernel<E, true>, grid, dim3(kRowsWarps * 32), 0, st, a) : launch_pdl(gqa_rows_kernel<E, false>, grid, dim3(kRowsWarps * 32), 0, st, a);
+  return (int)(int4 ? launch_pdl(gqa_rows_kernel<L, true>, grid, dim3(kRowsWarps * 32), 0, st, a) : launch_pdl(gqa_rows_kernel<L, false>, grid, dim3(kRowsWarps * 32), 0, st, a));
 }
 }  // namespace
 
-// qkv bf16 [T, (Hq + 2 Hkv) D], rows ld apart and aligned to 2 D / 32 bytes; positions int64 [axes, T], rows pos_ld apart; rope fp32 [max_pos, D] (cos | sin);
-// caches: int4 != 0: uint8 [blocks, Hkv, block_size (D/2 + D/32)], else bf16 [blocks, block_size, Hkv, D].  chunk: heads a warp takes one after the other.
+// qkv bf16 [T, (Hq + 2 Hkv) D], rows ld apart and aligned to 8 bytes; positions int64 [axes, T], rows pos_ld apart; rope fp32 [max_pos, D] (cos | sin);
+// caches: int4 != 0: uint8 [blocks, Hkv, block_size (D/2 + D/32)], else bf16 [blocks, block_size, Hkv, D].
 extern "C" int ne_gqa_rows(const void* qkv, long long ld, int Hq, int Hkv, int D, const void* qw, const void* kw, double eps, float w_offset, const long long* positions,
                            long long pos_ld, const float* rope, int max_pos, int axes, const int* sections, int interleaved, void* q_out, void* k_cache, void* v_cache,
-                           const long long* slots, long long cache_rows, int block_size, int int4, int chunk, int T, cudaStream_t st) {
+                           const long long* slots, long long cache_rows, int block_size, int int4, int T, cudaStream_t st) {
   if (T <= 0) return 0;
-  if (Hq < 0 || Hkv < 1 || axes < 1 || axes > 4 || max_pos < 1 || block_size < 1 || chunk < 1) return 1001;
+  if (Hq < 0 || Hkv < 1 || axes < 1 || axes > 4 || max_pos < 1 || block_size < 1) return 1001;
   RowsArgs a{};
   a.qkv = (const __nv_bfloat16*)qkv; a.ld = ld; a.qw = (const __nv_bfloat16*)qw; a.kw = (const __nv_bfloat16*)kw; a.eps = eps; a.w_offset = w_offset;
   a.positions = positions; a.pos_ld = pos_ld; a.rope = rope; a.max_pos = max_pos; a.axes = axes; a.interleaved = interleaved;
   for (int i = 0; i < axes; i++) a.sections[i] = sections[i];
   a.q_out = (__nv_bfloat16*)q_out; a.k_cache = (uint8_t*)k_cache; a.v_cache = (uint8_t*)v_cache; a.slots = slots; a.cache_rows = cache_rows;
-  a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.block_size = block_size; a.chunk = chunk;
+  a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.block_size = block_size;
+  // few rows: a warp per step, so that all SMs work; many: eight steps under one fetch of the angles
+  a.chunk = (long long)T * Hq * D >= 148ll * 64 * 256 * 4 ? 8 : 1;
   switch (D) {
-    case 32: return (int)launch_rows<1>(a, int4, st);
-    case 64: return (int)launch_rows<2>(a, int4, st);
-    case 128: return (int)launch_rows<4>(a, int4, st);
-    case 256: return (int)launch_rows<8>(a, int4, st);
+    case 32: return launch_rows<4>(a, int4, st);
+    case 64: return launch_rows<8>(a, int4, st);
+    case 128: return launch_rows<16>(a, int4, st);
+    case 256: return launch_rows<32>(a, int4, st);
     default: return 1002;
   }
 }
@@ -303,19 +365,14 @@ extern "C" int ne_gqa_rows(const void* qkv, long long ld, int Hq, int Hkv, int D
 extern "C" int ne_kv4_store(const void* k, const void* v, long long k_ld, long long v_ld, void* k_cache, void* v_cache, const long long* slots, long long cache_rows, int T,
                             int Hkv, int D, int block_size, cudaStream_t st) {
   if (T <= 0) return 0;
-  if (Hkv < 1 || block_size < 1) return 1001;
-  const dim3 grid((unsigned)(((long long)T * 2 * Hkv + kRowsWarps - 1) / kRowsWarps));
+  if (Hkv < 1 || block_size < 1 || (D != 32 && D != 64 && D != 128 && D != 256)) return 1001;
+  const int per_step = 256 / D, steps = (Hkv + per_step - 1) / per_step;
+  const dim3 grid((unsigned)(((long long)T * 2 * steps + kRowsWarps - 1) / kRowsWarps));
   auto go = [&](auto kern) {
     return (int)launch_pdl(kern, grid, dim3(kRowsWarps * 32), 0, st, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, k_ld, v_ld, (uint8_t*)k_cache, (uint8_t*)v_cache, slots,
                            cache_rows, T, Hkv, block_size);
   };
-  switch (D) {
-    case 32: return go(kv4_store_kernel<1>);
-    case 64: return go(kv4_store_kernel<2>);
-    case 128: return go(kv4_store_kernel<4>);
-    case 256: return go(kv4_store_kernel<8>);
-    default: return 1002;
-  }
+  return D == 32 ? go(kv4_store_kernel<4>) : D == 64 ? go(kv4_store_kernel<8>) : D == 128 ? go(kv4_store_kernel<16>) : go(kv4_store_kernel<32>);
 }
 
 extern "C" int ne_kv4_gather(const void* k_cache, const void* v_cache, const long long* slots, long long cache_rows, void* k_out, void* v_out, int T, int Hkv, int D,

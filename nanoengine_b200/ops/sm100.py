@@ -772,8 +772,7 @@ def _kv4_store(k_cache, v_cache, slot_mapping, k, v) -> None:
     _same_device(k, v, k_cache, v_cache, slot_mapping)
     if T == 0:
         return
-    al = dim // 32                       # elements a lane loads at once
-    k2, v2 = (t if t.stride(2) == 1 and t.stride(1) == dim and t.stride(0) % al == 0 and t.data_ptr() % (2 * al) == 0
+    k2, v2 = (t if t.stride(2) == 1 and t.stride(1) == dim and t.stride(0) % 4 == 0 and t.data_ptr() % 8 == 0
               else t.clone(memory_format=torch.contiguous_format) for t in (k, v))
     slots = _slots_of(slot_mapping, T)
     _ck(_fn("ne_kv4_store", "ppllpppliiiip")(
@@ -824,22 +823,19 @@ def _gqa_rows(qkv, hq, hkv, hd, q_norm_w, k_norm_w, eps, unit_offset, positions,
     slots = _slots_of(slot_mapping, T)
     if T == 0:
         return q
-    al = hd // 32
-    if qkv.stride(1) != 1 or qkv.stride(0) % al or qkv.data_ptr() % (2 * al):
+    if qkv.stride(1) != 1 or qkv.stride(0) % 4 or qkv.data_ptr() % 8:
         qkv = qkv.clone(memory_format=torch.contiguous_format)
     norms = []
     for w in (q_norm_w, k_norm_w):
         if w is not None and w.numel() != hd:
             raise ValueError(f"norm weights have {hd} values")
         w = None if w is None else w.to(torch.bfloat16).contiguous()
-        norms.append(w if w is None or w.data_ptr() % (2 * al) == 0 else w.clone())
+        norms.append(w if w is None or w.data_ptr() % 8 == 0 else w.clone())
     pos = positions if positions.dtype == torch.int64 and positions.stride(-1) == 1 else positions.long().contiguous()
-    heads = hq + 2 * hkv
-    chunk = 1
-    _ck(_fn("ne_gqa_rows", "pliiippdfplpiipippppliiiip")(
+    _ck(_fn("ne_gqa_rows", "pliiippdfplpiipippppliiip")(
         qkv.data_ptr(), qkv.stride(0), hq, hkv, hd, 0 if norms[0] is None else norms[0].data_ptr(), 0 if norms[1] is None else norms[1].data_ptr(), float(eps),
         1.0 if unit_offset else 0.0, pos.data_ptr(), pos.stride(0) if sections is not None else 0, rope_cache.data_ptr(), rope_cache.shape[0], len(sec),
-        (_c.c_int * len(sec))(*sec), 1 if interleaved else 0, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), rows, bs, 1 if int4 else 0, chunk, T,
+        (_c.c_int * len(sec))(*sec), 1 if interleaved else 0, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), rows, bs, 1 if int4 else 0, T,
         _stream()), "ne_gqa_rows")
     return q
 

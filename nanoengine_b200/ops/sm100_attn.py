@@ -282,14 +282,8 @@ def gqa_attention_paged(q, k_cache, v_cache, block_tables, cu_seqlens_q, context
     return out
 
 
-INT4_CALLS = [0]             # launches of the kernel that reads 4-bit pages itself
-
-
-def _int4_splits(ctas: int, tiles: int) -> int:
-    """Key slices of the 4-bit kernel."""
-    if ctas >= _sms():
-        return 1
-    return max(1, min(_sms() // ctas, tiles // 4, 32))
+INT4_CALLS = [0]             # calls of the kernel that reads 4-bit pages itself
+_INT4_SHARES = {}
 
 
 def _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale, window: int):
@@ -318,21 +312,20 @@ def _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, sca
     if T * g >= 128 * B and (g % 4 == 0 or g == 1 and Hq % 4 == 0) and g <= 128:
         k, v, bt, cl = _k.kv4_expand(k_cache, v_cache, bt, cl, D)
         return gqa_attention_paged(q, k, v, bt, cu, cl, scale, window)
-    tiles = min(T, T // tq + B)
-    ctas = tiles * Hkv * -(-g // 16)
-    keys = bt.shape[1] * bs if window <= 0 else min(bt.shape[1] * bs, window + tq + 62)
-    S = _int4_splits(ctas, -(-keys // 64))
-    part = lse2 = None
-    if S > 1:
-        part = torch.empty(S, T, Hq, D, dtype=torch.float32, device=q.device)
-        lse2 = torch.empty(S, T, Hq, dtype=torch.float32, device=q.device)
-    _k._ck(_k._fn("ne_gqa_int4", "plppiipli" + "ppi" + "iiiiiii" + "f" + "pppp")(
+    # equal shares of the batch's work, one for every warp that is resident at once, but no more than its tiles of keys need
+    per_sm = _INT4_SHARES.get(D)
+    if per_sm is None:
+        per_sm = _INT4_SHARES[D] = _k.lib().ne_gqa_int4_shares(D)
+    tiles = min(T, T // tq + B) * Hkv * -(-g // 16)
+    shares = min(_sms() * per_sm, -(-tiles * -(-bt.shape[1] * bs // (32 if D == 256 else 64)) // 8) * 4)
+    # partial results, their statistics and the row tiles that cuts run through
+    part = torch.empty(shares * 32 * (D + 1) + 4 * (tiles + 1), dtype=torch.float32, device=q.device)
+    at = part.data_ptr()
+    _k._ck(_k._fn("ne_gqa_int4", "plppiipli" + "ppi" + "iiiiiii" + "f" + "ppppp")(
         q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], bs, bt.data_ptr(), bt.stride(0), bt.shape[1], cu.data_ptr(), cl.data_ptr(), B,
-        T, Hq, Hkv, D, tiles, S, max(0, int(window)), scale, out.data_ptr(), 0 if part is None else part.data_ptr(), 0 if lse2 is None else lse2.data_ptr(), _k._stream()),
-        "ne_gqa_int4")
+        T, Hq, Hkv, D, shares, tiles, max(0, int(window)), scale, out.data_ptr(), at, at + shares * 128 * D, at + shares * 128 * (D + 1), _k._stream()), "ne_gqa_int4")
     INT4_CALLS[0] += 1
-    if S > 1:
-        _k._ck(_k.lib().ne_attn_merge(_k._p(part), _k._p(lse2), _k._p(out), _c.c_int(S), _c.c_longlong(T * Hq), _c.c_int(D), _c.c_int(D), _k._st()), "ne_attn_merge")
+    _k.LAUNCHES[0] += 1
     return out
 
 
