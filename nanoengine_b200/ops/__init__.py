@@ -46,4 +46,5 @@ def __getattr__(name):
         return ref_fn(*args, **kw)
 
     dispatch.__name__ = name
+    globals()[name] = dispatch            # the next lookup finds it without coming here
     return dispatch

@@ -735,26 +735,28 @@ def _fn(name: str, spec: str):
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
-def _same_device(first: torch.Tensor, *others) -> None:
+def _same_device(*tensors) -> None:
     """All of a call's tensors live on the current device: the kernels launch there."""
-    dev = first.device
-    if dev.type != "cuda" or dev.index != torch.cuda.current_device() or any(t is not None and t.device != dev for t in others):
-        raise ValueError("the tensors of a call live on the current CUDA device")
+    cur = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != cur:
+            raise ValueError("the tensors of a call live on the current CUDA device")
 
 
 def _kv4_dims(k_cache, v_cache, hkv: int, dim: int) -> int:
     """Block size of a pair of 4-bit caches the kernels can address."""
-    bs = ref.kv4_block_size(k_cache, dim)
     if dim not in KV4_DIMS:
         raise ValueError(f"4-bit rows on the GPU: head sizes {KV4_DIMS}, not {dim}")
-    if v_cache.dtype != torch.uint8 or v_cache.shape != k_cache.shape or k_cache.shape[1] != hkv:
-        raise ValueError(f"4-bit keys and values come in caches of one shape, of {hkv} kv heads")
-    if not (k_cache.is_contiguous() and v_cache.is_contiguous()) or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+    shape = k_cache.shape
+    row = dim // 2 + dim // 32
+    if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8 or v_cache.shape != shape or len(shape) != 3 or shape[1] != hkv or shape[2] % row or shape[2] < row:
+        raise ValueError(f"4-bit keys and values of heads of {dim} come in caches uint8 [blocks, {hkv}, block_size * {row}] of one shape")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()) or (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
         raise ValueError("4-bit caches are contiguous and aligned to 16 bytes")
-    return bs
+    return shape[2] // row
 
 
 def _slots_of(slot_mapping, T: int):
@@ -785,7 +787,7 @@ def gqa_kv_gather(k_cache, v_cache, slots, dim):
     T, hkv = slots.numel(), k_cache.shape[1]
     bs = _kv4_dims(k_cache, v_cache, hkv, dim)
     _same_device(k_cache, v_cache, slots)
-    k, v = (torch.empty(T, hkv, dim, dtype=torch.bfloat16, device=k_cache.device) for _ in range(2))
+    k, v = torch.empty(2, T, hkv, dim, dtype=torch.bfloat16, device=k_cache.device)
     if T:
         _ck(_fn("ne_kv4_gather", "ppplppiiiip")(k_cache.data_ptr(), v_cache.data_ptr(), _i64c(slots).data_ptr(), k_cache.shape[0] * bs, k.data_ptr(), v.data_ptr(), T, hkv, dim,
                                                 bs, _stream()), "ne_kv4_gather")
@@ -858,29 +860,31 @@ def kv4_expand(k_cache, v_cache, block_tables, context_lens, dim: int):
 
 def step_tables(q_lens, seq_lens, block_ids, block_offsets, block_size, num_tokens, max_blocks, rows=None, pad_len=1, scratch_block=-1, out=None):
     """One launch; every tensor int32 (other integers are converted)."""
-    B = q_lens.numel()
+    B, n_ids, i32 = q_lens.numel(), block_ids.numel(), torch.int32
     rows = ref._step_sizes(B, block_size, num_tokens, max_blocks, rows, pad_len, scratch_block)
     if seq_lens.numel() != B or block_offsets.numel() != B + 1:
         raise ValueError("step_tables: one length per sequence and one offset more")
     if rows > 12000:
         raise ValueError("step_tables: at most 12000 rows")
     _same_device(q_lens, seq_lens, block_ids, block_offsets)
-    dev = q_lens.device
-    q, n, ids, off = (t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous() for t in (q_lens, seq_lens, block_ids, block_offsets))
-    sizes = [(rows + 1,), (rows,), (num_tokens,), (num_tokens,), (rows, max_blocks), (rows,)]
+    if not (q_lens.dtype == seq_lens.dtype == block_ids.dtype == block_offsets.dtype == i32 and q_lens.is_contiguous() and seq_lens.is_contiguous()
+            and block_ids.is_contiguous() and block_offsets.is_contiguous()):
+        q_lens, seq_lens, block_ids, block_offsets = (t.to(i32).contiguous() for t in (q_lens, seq_lens, block_ids, block_offsets))
     if out is None:
-        i32, i64 = dict(dtype=torch.int32, device=dev), dict(dtype=torch.int64, device=dev)
-        made = StepTables(torch.empty(rows + 1, **i32), torch.empty(rows, **i32), torch.empty(num_tokens, **i64), torch.empty(num_tokens, **i64),
-                          torch.empty(rows, max_blocks, **i32), torch.empty(rows, **i32))
+        dev, i64, empty = q_lens.device, torch.int64, torch.empty
+        cu, ctx, last = empty(rows + 1, dtype=i32, device=dev), empty(rows, dtype=i32, device=dev), empty(rows, dtype=i32, device=dev)
+        pos, slot, table = empty(num_tokens, dtype=i64, device=dev), empty(num_tokens, dtype=i64, device=dev), empty(rows, max_blocks, dtype=i32, device=dev)
+        ld = max_blocks
     else:
+        sizes = [(rows + 1,), (rows,), (num_tokens,), (num_tokens,), (rows, max_blocks), (rows,)]
         ref._check_step_out(out, sizes)
-        _same_device(q_lens, *out)
-        made = StepTables(*(o[tuple(slice(k) for k in size)] for o, size in zip(out, sizes)))
+        _same_device(*out)
+        cu, ctx, pos, slot, table, last = (o[tuple(slice(k) for k in size)] for o, size in zip(out, sizes))
+        ld = max(table.stride(0), max_blocks)
     _ck(_fn("ne_step_tables", "pppp" + "iiiiiiii" + "ppppp" + "lpp")(
-        q.data_ptr(), n.data_ptr(), ids.data_ptr(), off.data_ptr(), B, rows, ids.numel(), int(block_size), int(num_tokens), int(max_blocks), int(pad_len), int(scratch_block),
-        made.cu_seqlens_q.data_ptr(), made.context_lens.data_ptr(), made.positions.data_ptr(), made.slot_mapping.data_ptr(), made.block_tables.data_ptr(),
-        made.block_tables.stride(0) if rows else int(max_blocks), made.last_token_indices.data_ptr(), _stream()), "ne_step_tables")
-    return made
+        q_lens.data_ptr(), seq_lens.data_ptr(), block_ids.data_ptr(), block_offsets.data_ptr(), B, rows, n_ids, block_size, num_tokens, max_blocks, pad_len, scratch_block,
+        cu.data_ptr(), ctx.data_ptr(), pos.data_ptr(), slot.data_ptr(), table.data_ptr(), ld, last.data_ptr(), _stream()), "ne_step_tables")
+    return StepTables(cu, ctx, pos, slot, table, last)
 
 
 # ---- MoE -----------------------------------------------------------------------------------------

@@ -289,9 +289,11 @@ _INT4_SHARES = {}
 def _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale, window: int):
     """4-bit pages: a kernel that unpacks them in registers for steps of few query rows per key, the tensor-core kernels over pages expanded to bf16 for others."""
     T, Hq, D = q.shape
-    Hkv, bs = _k.ref.check_kv4(q, k_cache, v_cache)
-    _k._kv4_dims(k_cache, v_cache, Hkv, D)
-    if D == 32 or not (bs in (16, 32) or bs % 64 == 0):
+    Hkv = k_cache.shape[1] if k_cache.dim() > 1 else 0
+    bs = _k._kv4_dims(k_cache, v_cache, Hkv, D)
+    if Hkv < 1 or Hq < Hkv or Hq % Hkv:
+        raise ValueError(f"{Hq} query heads over {Hkv} kv heads")
+    if D == 32 or not (bs == 16 or bs == 32 or bs % 64 == 0):
         raise ValueError(f"attention over 4-bit pages on the GPU: head sizes 64, 128 and 256, pages of 16, 32 or a multiple of 64 tokens, not {D} and {bs}")
     if not scale > 0:
         raise ValueError("the scale of the scores is positive")
@@ -300,15 +302,11 @@ def _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, sca
     if bt.dim() != 2 or bt.shape[0] < B or cu.numel() != B + 1:
         raise ValueError("one block table row per sequence, and one query boundary more")
     _k._same_device(q, k_cache, v_cache, bt, cu, cl)
-    out = torch.empty(T, Hq, D, dtype=torch.bfloat16, device=q.device)
-    if T == 0:
-        return out
-    if B == 0 or bt.shape[1] == 0:
-        return out.zero_()
-    q = q if q.dtype == torch.bfloat16 and q.stride(2) == 1 and q.stride(1) == D and q.stride(0) % 4 == 0 and q.data_ptr() % 8 == 0 else \
-        q.to(torch.bfloat16).clone(memory_format=torch.contiguous_format)
-    g = Hq // Hkv
-    tq = max(1, 16 // g)
+    W, g, dev = bt.shape[1], Hq // Hkv, q.device
+    if T == 0 or B == 0 or W == 0:
+        return torch.zeros(T, Hq, D, dtype=torch.bfloat16, device=dev)
+    if q.dtype != torch.bfloat16 or q.stride(2) != 1 or q.stride(1) != D or q.stride(0) % 4 or q.data_ptr() % 8:
+        q = q.to(torch.bfloat16).clone(memory_format=torch.contiguous_format)
     if T * g >= 128 * B and (g % 4 == 0 or g == 1 and Hq % 4 == 0) and g <= 128:
         k, v, bt, cl = _k.kv4_expand(k_cache, v_cache, bt, cl, D)
         return gqa_attention_paged(q, k, v, bt, cu, cl, scale, window)
@@ -316,14 +314,16 @@ def _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, sca
     per_sm = _INT4_SHARES.get(D)
     if per_sm is None:
         per_sm = _INT4_SHARES[D] = _k.lib().ne_gqa_int4_shares(D)
+    tq = 16 // g if g < 16 else 1
     tiles = min(T, T // tq + B) * Hkv * -(-g // 16)
-    shares = min(_sms() * per_sm, -(-tiles * -(-bt.shape[1] * bs // (32 if D == 256 else 64)) // 8) * 4)
+    shares = min(_sms() * per_sm, -(-tiles * -(-W * bs // (32 if D == 256 else 64)) // 8) * 4)
+    out = torch.empty(T, Hq, D, dtype=torch.bfloat16, device=dev)
     # partial results, their statistics and the row tiles that cuts run through
-    part = torch.empty(shares * 32 * (D + 1) + 4 * (tiles + 1), dtype=torch.float32, device=q.device)
+    part = torch.empty(shares * 32 * (D + 1) + 4 * (tiles + 1), dtype=torch.float32, device=dev)
     at = part.data_ptr()
     _k._ck(_k._fn("ne_gqa_int4", "plppiipli" + "ppi" + "iiiiiii" + "f" + "ppppp")(
-        q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], bs, bt.data_ptr(), bt.stride(0), bt.shape[1], cu.data_ptr(), cl.data_ptr(), B,
-        T, Hq, Hkv, D, shares, tiles, max(0, int(window)), scale, out.data_ptr(), at, at + shares * 128 * D, at + shares * 128 * (D + 1), _k._stream()), "ne_gqa_int4")
+        q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], bs, bt.data_ptr(), bt.stride(0), W, cu.data_ptr(), cl.data_ptr(), B,
+        T, Hq, Hkv, D, shares, tiles, window if window > 0 else 0, scale, out.data_ptr(), at, at + shares * 128 * D, at + shares * 128 * (D + 1), _k._stream()), "ne_gqa_int4")
     INT4_CALLS[0] += 1
     _k.LAUNCHES[0] += 1
     return out
