@@ -45,7 +45,7 @@ class Config:
     # the scales themselves; one setting per process.
     fp8_scale_format: str = "auto"
     # cache
-    kv_cache_dtype: str = "auto"             # auto | bfloat16 | fp8
+    kv_cache_dtype: str = "auto"             # auto | bfloat16 | fp8 | int4 (4-bit key / value rows of the GQA families)
     kvcache_block_size: int = 256
     num_kvcache_blocks: Optional[int] = None  # None = size from free memory
     gpu_memory_utilization: float = 0.9
@@ -113,8 +113,8 @@ class Config:
             raise ValueError(f"unknown routing_strategy {self.routing_strategy}")
         if self.fp8_scale_format not in ("auto", "fp32", "ue8m0"):
             raise ValueError("fp8_scale_format must be auto, fp32 or ue8m0")
-        if self.kv_cache_dtype not in ("auto", "bfloat16", "float32", "fp8"):
-            raise ValueError("kv_cache_dtype must be auto, bfloat16, float32 or fp8")
+        if self.kv_cache_dtype not in ("auto", "bfloat16", "float32", "fp8", "int4"):
+            raise ValueError("kv_cache_dtype must be auto, bfloat16, float32, fp8 or int4")
         if self.dtype not in ("bfloat16", "float16", "float32"):
             raise ValueError("dtype must be bfloat16, float16 or float32")
         if mc.is_mla:
@@ -125,6 +125,15 @@ class Config:
                 raise ValueError("MLA architectures run attention data-parallel: attention_tp must be 1")
         elif self.kvcache_block_size == 256:
             self.kvcache_block_size = 64
+        if self.kv_cache_dtype == "int4":
+            if mc.is_mla or mc.is_dsv4 or mc.layer_specs or mc.num_kv_shared_layers or mc.global_head_dim:
+                raise ValueError("kv_cache_dtype='int4' is offered for the GQA families with one head dim and one page tensor per layer")
+            if mc.head_dim % 32:
+                raise ValueError("a 4-bit cache keeps one scale per 32 dims: head_dim must be a multiple of 32")
+            if self.device != "cpu":
+                bs = self.kvcache_block_size
+                if mc.head_dim not in (64, 128, 256) or self.dtype != "bfloat16" or bs not in (16, 32) and bs % 64:
+                    raise ValueError("on the GPU a 4-bit cache needs head_dim 64, 128 or 256, dtype bfloat16 and kvcache_block_size 16, 32 or a multiple of 64")
         if self.attention_sp != 1:
             raise ValueError("attention_sp > 1 is not supported by the runner")
         spec = self.parallel_spec()

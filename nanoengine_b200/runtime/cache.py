@@ -3,7 +3,8 @@
 MLA latent cache   [L, blocks, block_size, R + rope]   bf16/fp32, or fp8 e4m3 raw rows (576 B per token per layer
                                                         for DeepSeek-V3: clamped cast, no scales)
 indexer key cache  [L, blocks, block_size * (D + 4)] u8 per page: block_size fp8 keys, then block_size fp32 scales
-GQA cache          [2, L, blocks, block_size, kv_heads_local, head_dim]
+GQA cache          [2, L, blocks, block_size, kv_heads_local, head_dim]; in 4 bits [2, L, blocks, kv_heads_local, page bytes] u8: per
+                   page and head the codes of block_size tokens, then their scale bytes (`ops.kv4_page_bytes`)
 recurrent state    hybrid models with gated delta-net layers keep, per sequence slot and linear layer, the delta-rule state
                    [Hv, Dv, Dk] fp32 and the convolution window [K-1, conv_dim]; the paged GQA cache then covers only the
                    full-attention layers.  Slot `state_slots` (one past the scheduler-visible range) is scratch.
@@ -41,7 +42,7 @@ from ..models.config import ModelConfig
 
 
 def torch_dtype(name: str):
-    return {"bfloat16": torch.bfloat16, "float16": torch.float16, "float32": torch.float32, "fp8": torch.float8_e4m3fn}[name]
+    return {"bfloat16": torch.bfloat16, "float16": torch.float16, "float32": torch.float32, "fp8": torch.float8_e4m3fn, "int4": torch.uint8}[name]
 
 
 @dataclass
@@ -79,6 +80,7 @@ class CachePlan:
     kv_shapes: Optional[List[tuple]] = None
     delta_shapes: Optional[List[tuple]] = None
     pools: Optional[List[int]] = None          # tokens per pooled row of every layer in kv_shapes (0: the layer does not pool)
+    int4: bool = False                         # GQA rows in 4 bits (kv_dtype is the stored type, uint8)
     hisparse: bool = False
     hot_rows: int = 0
     hs_slots: int = 0
@@ -104,6 +106,12 @@ class CachePlan:
         return pooled_rows_per_page(p, self.block_size) if p else 0
 
     @property
+    def page_bytes(self) -> int:
+        """4-bit rows: bytes one page takes per key / value head."""
+        from ..ops.reference import kv4_page_bytes
+        return kv4_page_bytes(self.row_dim, self.block_size)
+
+    @property
     def needs_state_slots(self) -> bool:
         return self.gdn or self.dsv4
 
@@ -117,7 +125,7 @@ class CachePlan:
             return sum(2 * 4 * (2 if r == 4 else 1) ** 2 * r * self.dsv4_head_dim for r in self.dsv4_ratios if r)
         if not self.gdn:
             return 0
-        e = 2 if self.kv_dtype in (torch.bfloat16, torch.float16, torch.float8_e4m3fn) else 4
+        e = 2 if self.int4 or self.kv_dtype in (torch.bfloat16, torch.float16, torch.float8_e4m3fn) else 4
         if self.delta_shapes is not None:
             return sum(h * dv * dk * 4 + (k - 1) * c * e for h, dv, dk, k, c in self.delta_shapes)
         return self.gdn_layers * (self.gdn_heads * self.gdn_dv * self.gdn_dk * 4 + (self.conv_k - 1) * self.conv_dim * e)
@@ -137,6 +145,8 @@ class CachePlan:
             return sum((self.block_size + self.pooled_rows(l)) * g * (d + dv) for l, (g, d, dv) in enumerate(self.kv_shapes)) * e
         if self.mla:
             return self.num_layers * self.block_size * self.row_dim * e
+        if self.int4:
+            return 2 * self.num_layers * self.kv_heads_local * self.page_bytes
         return 2 * self.num_layers * self.block_size * self.kv_heads_local * self.row_dim * e
 
     @property
@@ -178,6 +188,9 @@ def make_cache_plan(mc: ModelConfig, kv_dtype_name: str, block_size: int, attn_t
     if hisparse_rows:
         assert plan.mla and plan.indexer, "the hot / cold tier needs an MLA cache with the DSA indexer"
         plan.hisparse, plan.hot_rows, plan.hs_slots, plan.max_ctx = True, hisparse_rows, state_slots, max_ctx
+    if kv_dtype_name == "int4":
+        assert plan.gqa and not plan.listed and not plan.layer_dims, "4-bit rows are kept by the GQA families with one head dim"
+        plan.int4 = True
     return plan
 
 
@@ -282,7 +295,9 @@ class KVCache:
                 self.kv = self.kv.view(torch.float8_e4m3fn)
             self.layers = [self.kv[l] for l in range(plan.num_layers)]
         else:
-            self.kv = torch.zeros(2, plan.num_layers, nb, plan.block_size, plan.kv_heads_local, plan.row_dim, dtype=plan.kv_dtype, device=device)
+            # a zeroed 4-bit page holds the lowest code times the smallest scale, finite like every other pair of code and scale byte
+            shape = (plan.kv_heads_local, plan.page_bytes) if plan.int4 else (plan.block_size, plan.kv_heads_local, plan.row_dim)
+            self.kv = torch.zeros(2, plan.num_layers, nb, *shape, dtype=plan.kv_dtype, device=device)
             self.layers = [(self.kv[0, l], self.kv[1, l]) for l in range(plan.num_layers)]
             if plan.layer_dims:
                 def front(t, d):          # a contiguous [blocks, block_size, heads, d] cache at the front of the layer's slab
@@ -315,7 +330,7 @@ class KVCache:
         self.rec_states = self.conv_states = None
         self.scratch_slot = plan.state_slots
         ns = plan.state_slots + 1       # + scratch slot for padded graph rows and dummy batches
-        cdt = torch.bfloat16 if plan.kv_dtype == torch.float8_e4m3fn else plan.kv_dtype
+        cdt = torch.bfloat16 if plan.int4 or plan.kv_dtype == torch.float8_e4m3fn else plan.kv_dtype
         if plan.delta_shapes is not None:
             self.rec = self.conv = None
             self.rec_states = [torch.zeros(ns, h, dv, dk, dtype=torch.float32, device=device) for h, dv, dk, _, _ in plan.delta_shapes]
