@@ -134,6 +134,8 @@ class Config:
                 bs = self.kvcache_block_size
                 if mc.head_dim not in (64, 128, 256) or self.dtype != "bfloat16" or bs not in (16, 32) and bs % 64:
                     raise ValueError("on the GPU a 4-bit cache needs head_dim 64, 128 or 256, dtype bfloat16 and kvcache_block_size 16, 32 or a multiple of 64")
+        if mc.position_axes is not None and (len(mc.position_axes) != 3 or min(mc.position_axes) < 0 or sum(mc.position_axes) * 2 != mc.head_dim):
+            raise ValueError(f"mrope_section {mc.position_axes}: the angles of time, row and column, half of head_dim {mc.head_dim} together")
         if self.attention_sp != 1:
             raise ValueError("attention_sp > 1 is not supported by the runner")
         spec = self.parallel_spec()

@@ -54,6 +54,35 @@ static py::dict prepare_runner_inputs(const Batch& b, int block_size, int pad_bl
   return d;
 }
 
+// The same step as one int32 array for a worker that builds the tables on its device: q_lens [n], seq_lens [n], block offsets [n + 1], the page lists
+// and the token ids, behind one another.  `consecutive` says whether every token stands where the lengths alone put it.
+static py::dict pack_runner_inputs(const Batch& b, int block_size) {
+  const size_t n = b.num_seqs(), ids = b.block_tables.size(), T = b.input_ids.size();
+  std::vector<int32_t> cu_q(n + 1, 0);
+  int max_blocks = 1, max_q = 0, max_k = 0;
+  if (b.positions.size() != T || b.q_lens.size() != n || b.seq_lens.size() != n || b.block_offsets.size() != n + 1)
+    throw std::runtime_error("prepare: the lengths of the step's lists disagree");
+  bool consecutive = true;
+  size_t t = 0;
+  for (size_t i = 0; i < n; i++) {
+    const int q = b.q_lens[i], k = b.seq_lens[i], nb = b.block_offsets[i + 1] - b.block_offsets[i];
+    cu_q[i + 1] = cu_q[i] + q;
+    max_blocks = std::max(max_blocks, nb); max_q = std::max(max_q, q); max_k = std::max(max_k, k);
+    for (int j = 0; j < q && t < T; j++, t++) {
+      if (b.positions[t] / block_size >= nb) throw std::runtime_error("prepare: position beyond the sequence's block table");
+      consecutive &= b.positions[t] == k - q + j;
+    }
+  }
+  py::array_t<int32_t> packed((py::ssize_t)(3 * n + 1 + ids + T));
+  int32_t* p = packed.mutable_data();
+  for (const std::vector<int32_t>* v : {&b.q_lens, &b.seq_lens, &b.block_offsets, &b.block_tables, &b.input_ids}) p = std::copy(v->begin(), v->end(), p);
+  py::dict d;
+  d["packed"] = packed; d["num_ids"] = ids; d["consecutive"] = consecutive && t == T;
+  d["cu_seqlens_q"] = to_np(cu_q); d["context_lens"] = to_np(b.seq_lens); d["max_blocks"] = max_blocks;
+  d["max_seqlen_q"] = max_q; d["max_seqlen_k"] = max_k;
+  return d;
+}
+
 PYBIND11_MODULE(_core, m) {
   m.doc() = "nanoengine_b200 native control plane: scheduler, block manager, wire codec, metrics";
   py::register_exception<WireError>(m, "WireError", PyExc_ValueError);
@@ -151,6 +180,7 @@ PYBIND11_MODULE(_core, m) {
       .def_readwrite("swap_out_dst", &Batch::swap_out_dst)
       .def_property_readonly("num_seqs", &Batch::num_seqs)
       .def("prepare", &prepare_runner_inputs, py::arg("block_size"), py::arg("pad_blocks_to") = 0)
+      .def("pack", &pack_runner_inputs, py::arg("block_size"))
       .def("to_bytes", [](const Batch& b) { return py::bytes(b.to_bytes()); })
       .def_static("from_bytes", [](const std::string& b) { return Batch::from_bytes(b); });
 

@@ -31,6 +31,7 @@ struct I4Args {
   const int* block_tables; long long bt_ld; int bt_width;
   const int* cu_seqlens_q; const int* context_lens; int num_seqs;
   int T, Hq, Hkv, g, tq, head_tiles, window, shares;   // tq tokens x min(g, 16) heads a row tile; head_tiles = ceil(g / 16)
+  int max_tiles;                                       // places in cuts
   float scale_log2;
   __nv_bfloat16* out;                                  // [T, Hq, D]
   float* part; float* lse2;                            // [shares, 2, 16, D], [shares, 2, 16]
@@ -58,7 +59,7 @@ struct I4Seq { int q_beg, q_len, ctx, first, per_tile, tiles; };        // first
 template <int KEYS> __device__ __forceinline__ I4Seq i4_seq(const I4Args& a, int q_beg, int q_end, int ctx) {
   I4Seq s;
   s.q_beg = q_beg;
-  s.q_len = max(0, q_end - q_beg);
+  s.q_len = min(max(0, q_end - q_beg), a.T);
   s.ctx = (int)max(0ll, min((long long)ctx, (long long)a.bt_width * a.block_size));
   const int first_key = a.window > 0 ? max(0, s.ctx - s.q_len - a.window + 1) : 0;
   s.first = first_key / KEYS;
@@ -71,53 +72,66 @@ template <int KEYS> __device__ __forceinline__ I4Seq i4_load(const I4Args& a, in
 }
 
 // Units of a share: equal ones, but no less than two
-__device__ __forceinline__ int i4_share(int total, int shares) { return max((total + shares - 1) / shares, 2); }
+__device__ __forceinline__ int i4_share(long long total, int shares) { return (int)max((total + shares - 1) / shares, 2ll); }
 
 constexpr int kI4MaxSlots = 3;
 struct I4Shared {
   uint64_t bar[kI4Warps * kI4MaxSlots];                                  // a slot's tile has landed
   uint32_t bad[kI4Warps * kI4MaxSlots];                                  // pieces of it whose page lies outside the cache
-  int abort, warp[2 * kI4Warps];
-  int4 start[kI4Warps];                                                  // sequence that a warp's share starts in; units and row tiles in front of it
+  int abort, tiles[kI4Warps];
+  long long units[kI4Warps];
+  int4 start[kI4Warps];                                                  // where a warp's share starts: sequence, (row tile, head) of it, unit of that; row tiles in front of the sequence
   int beg[kI4Threads], end[kI4Threads], ctx[kI4Threads];                 // what the sequences from the first of these on are
 };
 
-// Totals (units, row tiles), and where the shares of this CTA's warps start.  All threads of the CTA, each with a run of sequences.
-template <int KEYS> __device__ __forceinline__ int2 i4_plan(const I4Args& a, I4Shared& sh, int& share) {
+// Totals (units, row tiles), and where the shares of this CTA's warps start.  All threads of the CTA, each with a run of sequences.  (Units are counted in 64
+// bits: a prompt of 262144 tokens has 3 10^9 of them where three tokens make a row tile.)
+struct I4Total { long long units; int tiles, share; };
+template <int KEYS> __device__ __forceinline__ I4Total i4_plan(const I4Args& a, I4Shared& sh) {
   const int run = (a.num_seqs + kI4Threads - 1) / kI4Threads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int s0 = threadIdx.x * run, s1 = min(a.num_seqs, s0 + run), heads = a.Hkv * a.head_tiles;
-  int mine = 0, tiles = 0;
+  long long mine = 0;
+  int tiles = 0;
   for (int i = s0; i < s1; i++) {
     const I4Seq s = i4_load<KEYS>(a, i);
     tiles += s.tiles * heads;
-    mine += s.tiles * heads * s.per_tile;
+    mine += (long long)s.tiles * heads * s.per_tile;
   }
-  int incl = mine, incl_t = tiles;
+  long long incl = mine;
+  int incl_t = tiles;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o), t = __shfl_up_sync(0xffffffffu, incl_t, o);
+    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    const int t = __shfl_up_sync(0xffffffffu, incl_t, o);
     if (lane >= o) { incl += v; incl_t += t; }
   }
-  if (lane == 31) { sh.warp[warp] = incl; sh.warp[kI4Warps + warp] = incl_t; }
+  if (lane == 31) { sh.units[warp] = incl; sh.tiles[warp] = incl_t; }
   __syncthreads();
-  int before = incl - mine, before_t = incl_t - tiles;
-  int2 total = make_int2(0, 0);
+  long long before = incl - mine;
+  int before_t = incl_t - tiles;
+  I4Total total = {0, 0, 0};
 #pragma unroll
   for (int w = 0; w < kI4Warps; w++) {
-    if (w < warp) { before += sh.warp[w]; before_t += sh.warp[kI4Warps + w]; }
-    total.x += sh.warp[w]; total.y += sh.warp[kI4Warps + w];
+    if (w < warp) { before += sh.units[w]; before_t += sh.tiles[w]; }
+    total.units += sh.units[w]; total.tiles += sh.tiles[w];
   }
-  share = i4_share(total.x, a.shares);
+  total.share = i4_share(total.units, a.shares);
 #pragma unroll
   for (int w = 0; w < kI4Warps; w++) {                                   // the thread whose run a share starts in finds the sequence
-    const long long u = ((long long)blockIdx.x * kI4Warps + w) * share;
+    const long long u = ((long long)blockIdx.x * kI4Warps + w) * total.share;
     if (u < before || u >= before + mine) continue;
-    int base = before, t = before_t;
+    long long base = before;
+    int t = before_t;
     for (int i = s0;; i++) {
       const I4Seq s = i4_load<KEYS>(a, i);
       const int n = s.tiles * heads;
-      if (u < base + n * s.per_tile || i + 1 >= s1) { sh.start[w] = make_int4(i, base, t, 0); break; }
-      base += n * s.per_tile;
+      const long long end = base + (long long)n * s.per_tile;
+      if (u < end || i + 1 >= s1) {
+        const int th = (int)((u - base) / s.per_tile);
+        sh.start[w] = make_int4(i, th, (int)(u - base - (long long)th * s.per_tile), t);
+        break;
+      }
+      base = end;
       t += n;
     }
   }
@@ -142,15 +156,15 @@ template <int KEYS> __device__ __forceinline__ void i4_fill(const I4Args& a, I4P
   p.t_begin = max(p.s.first + p.unit, low);
   p.t_end = p.n_tok > 0 ? min(p.s.first + p.unit + p.units, max_limit >= 0 ? max_limit / KEYS + 1 : 0) : 0;
 }
-// the piece that starts at unit u, in the sequence that `at` names; `left` units of the share remain
-template <int KEYS> __device__ __forceinline__ I4Piece i4_first(const I4Args& a, const int4& at, int u, int left) {
+// the piece that a share starts with; `left` units the share has
+template <int KEYS> __device__ __forceinline__ I4Piece i4_first(const I4Args& a, const int4& at, int left) {
   I4Piece p;
   p.seq = at.x;
   p.s = i4_load<KEYS>(a, p.seq);
-  const int heads = a.Hkv * a.head_tiles, th = (u - at.y) / p.s.per_tile, head = th % heads;
-  p.unit = u - at.y - th * p.s.per_tile;
-  p.index = at.z + th;
-  p.tile = th / heads;
+  const int heads = a.Hkv * a.head_tiles, head = at.y % heads;
+  p.unit = at.z;
+  p.index = at.w + at.y;
+  p.tile = at.y / heads;
   p.hkv = head / a.head_tiles;
   p.ht = head - p.hkv * a.head_tiles;
   i4_fill<KEYS>(a, p, left);
@@ -208,16 +222,16 @@ __global__ void __launch_bounds__(kI4Threads, I4Geo<D>::ctas) gqa_int4_kernel(co
     mbar_fence_init();
   }
   pdl_wait(); pdl_trigger();
-  int share;
-  const int2 total = i4_plan<G::keys>(a, sh, share);                     // (its barriers also publish the initialised mbarriers)
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.cuts[0] = make_int4(total.y, 0, 0, 0);
-  if ((long long)blockIdx.x * kI4Warps * share >= total.x) return;
+  const I4Total total = i4_plan<G::keys>(a, sh);                         // (its barriers also publish the initialised mbarriers)
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.cuts[0] = make_int4(total.tiles, 0, 0, 0);
+  const int share = total.share;
+  if ((long long)blockIdx.x * kI4Warps * share >= total.units) return;
   if (const int i = sh.start[0].x + threadIdx.x; i < a.num_seqs) {
     sh.beg[threadIdx.x] = a.cu_seqlens_q[i]; sh.end[threadIdx.x] = a.cu_seqlens_q[i + 1]; sh.ctx[threadIdx.x] = a.context_lens[i];
   }
   const int mine = blockIdx.x * kI4Warps + warp;                         // this warp's share
   const long long u0 = (long long)mine * share;
-  int left = (int)min((long long)share, max(0ll, total.x - u0));         // units of it still to do
+  int left = (int)min((long long)share, max(0ll, total.units - u0));         // units of it still to do
   uint8_t* ring = smem + warp * G::warp_bytes;
   uint64_t* bars = sh.bar + warp * ST;
   const uint32_t page_bytes = (uint32_t)a.block_size * (G::row + G::srow), id_bytes = a.Hkv * page_bytes;      // of one head, of a page id
@@ -275,7 +289,7 @@ __global__ void __launch_bounds__(kI4Threads, I4Geo<D>::ctas) gqa_int4_kernel(co
   };
 
   I4Piece p;
-  if (left > 0) p = i4_first<G::keys>(a, sh.start[warp], (int)u0, left);
+  if (left > 0) p = i4_first<G::keys>(a, sh.start[warp], left);
   __syncthreads();                                                       // the table of sequences
   if (left == 0) return;
   int slot = 0, phase = 0;                                               // of the next tile to read
@@ -454,8 +468,8 @@ __global__ void __launch_bounds__(kI4Threads, I4Geo<D>::ctas) gqa_int4_kernel(co
 
     // what follows this piece, and its first copies
     const bool whole = p.units == p.s.per_tile, head = p.unit == 0;
-    if (head && lane == 0) {                                             // the row tile's entry for the join: rows, first share with a piece of it, pieces
-      const int pieces = (int)((u0 + (min((long long)share, total.x - u0) - left) + p.s.per_tile - 1) / share) - mine + 1;
+    if (head && lane == 0 && p.index < a.max_tiles) {                                      // the row tile's entry for the join: rows, first share with a piece of it, pieces
+      const int pieces = (int)((u0 + (min((long long)share, total.units - u0) - left) + p.s.per_tile - 1) / share) - mine + 1;
       a.cuts[1 + p.index] = make_int4(tok0, max(0, n_tok * gh) | gh << 8 | pieces << 16, head0, mine);
     }
     left -= p.units;
@@ -600,7 +614,7 @@ extern "C" int ne_gqa_int4(const void* q, long long q_ld, const void* k, const v
   I4Args a{};
   a.q = (const __nv_bfloat16*)q; a.q_ld = q_ld; a.k = (const uint8_t*)k; a.v = (const uint8_t*)v; a.num_blocks = num_blocks; a.block_size = block_size;
   a.block_tables = block_tables; a.bt_ld = bt_ld; a.bt_width = bt_width; a.cu_seqlens_q = cu_seqlens_q; a.context_lens = context_lens; a.num_seqs = num_seqs;
-  a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.g = Hq / Hkv; a.tq = a.g >= 16 ? 1 : 16 / a.g; a.head_tiles = (a.g + 15) / 16; a.shares = shares;
+  a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.g = Hq / Hkv; a.tq = a.g >= 16 ? 1 : 16 / a.g; a.head_tiles = (a.g + 15) / 16; a.shares = shares; a.max_tiles = tiles;
   a.window = window > 0 ? window : 0; a.scale_log2 = scale * 1.4426950408889634f;
   a.out = (__nv_bfloat16*)out; a.part = part; a.lse2 = lse2; a.cuts = (int4*)cuts;
   switch (D) {

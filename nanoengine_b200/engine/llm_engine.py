@@ -85,6 +85,7 @@ class LLMEngine:
         self.scheduler = C.Scheduler(build_scheduler_config(config, self.num_blocks, plan.plan_bits()))
         self.executor.collective_rpc("allocate_kvcache", self.num_blocks)
         self._next_seq_id = 1
+        self._with_axes = set()        # requests whose workers keep image positions for them
         self.migrator = None   # set by the PD layer (disagg.KVMigrator)
         self.endpoint = None   # ZMQ endpoint of the engine process serving this engine, once it has one (published with the description)
         self._pd_connect = None        # connector of a prefill engine found through the control plane (tests substitute it)
@@ -124,14 +125,22 @@ class LLMEngine:
         return self.scheduler.add_request(C.RequestIn(seq_id, list(prompt_token_ids), sp, affinity_key))
 
     def add_vision_request(self, prompt_token_ids: List[int], image_token_id: int, embeddings=None, vision_slot=None, pool_desc=None,
-                           sampling_params=None, seq_id: Optional[int] = None) -> int:
+                           sampling_params=None, seq_id: Optional[int] = None, grid_thw=None, spatial_merge_size: int = 2) -> int:
         """A request whose `image_token_id` prompt tokens stand for image embeddings: given directly ([n, hidden]) or as a slot of
         a vision encoder's pool (`vl.EncoderEngine.encode` + `engine_info()["pool"]`).  The workers splice the rows in during
-        prefill.  Parity: reference engine/llm_component.py:285-340 + runtime/runner/model_runner.py:1557-1573, :1886-1890."""
+        prefill.  A model whose rotary positions have several axes places them by the images' patches, `grid_thw` [[t, h, w], ...] (the slot's own when
+        it has them); `spatial_merge_size` patches a side make one token.  Parity: reference engine/llm_component.py:285-340 + runtime/runner/model_runner.py:1557-1573, :1886-1890."""
         if seq_id is None:
             seq_id = self._next_seq_id
         slot, ntok = (int(vision_slot.slot), int(vision_slot.num_tokens)) if vision_slot is not None else (-1, 0)
-        self.executor.collective_rpc("register_vision", seq_id, list(prompt_token_ids), int(image_token_id), embeddings, pool_desc, slot, ntok)
+        grids = [list(g) for g in (grid_thw if grid_thw is not None else getattr(vision_slot, "grid_thw", None) or [])]
+        axes = bool(grids) and self.config.model_config.position_axes is not None
+        if axes and self.config.mode != "hybrid":
+            raise ValueError("image positions on several axes stay with the worker that ran the prompt: use mode='hybrid'")
+        self.executor.collective_rpc("register_vision", seq_id, list(prompt_token_ids), int(image_token_id), embeddings, pool_desc, slot, ntok,
+                                     grids if axes else None, int(spatial_merge_size))
+        if axes:
+            self._with_axes.add(seq_id)
         self._next_seq_id = max(self._next_seq_id, seq_id) + 1
         sp = sampling_params or C.SamplingParams()
         return self.scheduler.add_request(C.RequestIn(seq_id, list(prompt_token_ids), sp, 0, [slot] if slot >= 0 else None))
@@ -171,7 +180,13 @@ class LLMEngine:
             self.executor.collective_rpc("l3_store", pairs)
 
     def abort(self, seq_id: int) -> bool:
+        if seq_id in self._with_axes:
+            self._release_axes(seq_id)
         return self.scheduler.abort(seq_id)
+
+    def _release_axes(self, seq_id: int) -> None:
+        self._with_axes.discard(seq_id)
+        self.executor.collective_rpc("release_vision", seq_id)
 
     def is_finished(self) -> bool:
         return self.scheduler.is_finished()
@@ -195,6 +210,10 @@ class LLMEngine:
             outs = self.executor.run_batches(self.scheduler.serialize_run_batches())
         ms = (time.perf_counter() - t0) * 1e3
         step_outs = self.scheduler.postprocess_runner_out_bytes(outs, ms)
+        if self._with_axes:
+            for o in step_outs:
+                if o.seq_id in self._with_axes and o.status == C.FINISHED:
+                    self._release_axes(o.seq_id)
         if self.l3_enabled:
             self._l3_persist()
         every = self.config.status_log_interval_s

@@ -56,6 +56,9 @@ class ModelConfig:
     # GQA extras (Qwen3)
     qk_norm: bool = False
     attention_bias: bool = False
+    # rotary positions on several axes (time, height, width of image tokens): angles of each axis, in a row or interleaved
+    mrope_section: Optional[List[int]] = None
+    mrope_interleaved: bool = False
     # DSA lightning indexer (DeepSeek-V3.2)
     index_n_heads: int = 0
     index_head_dim: int = 128
@@ -169,6 +172,11 @@ class ModelConfig:
             return "sliding_attention"
         return "full_attention"
 
+    @property
+    def position_axes(self) -> Optional[List[int]]:
+        """Angles per axis of a model whose rotary positions have a time, a row and a column; None: one position per token."""
+        return self.mrope_section if self.architecture in ("Qwen3MoeForCausalLM", "Qwen3ForCausalLM") else None
+
     def attn_head_dim(self, layer_idx: int) -> int:
         return self.global_head_dim if (self.global_head_dim and self.attn_layer_type(layer_idx) == "full_attention") else self.head_dim
 
@@ -278,6 +286,10 @@ class ModelConfig:
         if isinstance(rp, dict):
             d.setdefault("rope_theta", rp.get("rope_theta", 10000000.0))
             d.setdefault("partial_rotary_factor", rp.get("partial_rotary_factor", 1.0))
+        for r in (rp, d.get("rope_scaling")):
+            if isinstance(r, dict) and r.get("mrope_section"):
+                d.setdefault("mrope_section", [int(n) for n in r["mrope_section"]])
+                d.setdefault("mrope_interleaved", bool(r.get("mrope_interleaved", False)))
         archs = d.pop("architectures", None)
         if archs and "architecture" not in d:
             d["architecture"] = archs[0]

@@ -56,7 +56,7 @@ class Qwen3Attention(nn.Module):
         # head split, q / k RMSNorm, rotary embedding and the paged K / V store in one pass over the projection output
         q = ops.gqa_qkv_prepare(qkv, self.hq, self.hkv, self.hd, self.q_norm.weight if self.q_norm is not None else None,
                                 self.k_norm.weight if self.k_norm is not None else None, self.cfg.rms_norm_eps, False, positions, rope_cache,
-                                kc, vc, ctx.slot_mapping)
+                                kc, vc, ctx.slot_mapping, self.cfg.position_axes, self.cfg.mrope_interleaved)
         o = ops.gqa_attention_paged(q, kc, vc, ctx.block_tables, ctx.cu_seqlens_q, ctx.context_lens, self.scale)
         o = o.reshape(T, self.hq * self.hd)
         return tp_linear_reduce_scatter(o, self.o_proj) if self.tp > 1 else self.o_proj(o)

@@ -858,14 +858,17 @@ def kv4_expand(k_cache, v_cache, block_tables, context_lens, dim: int):
     return k, v, bt, cl
 
 
+STEP_ROWS = 12000          # the kernel keeps the running sum of the lengths in shared memory
+
+
 def step_tables(q_lens, seq_lens, block_ids, block_offsets, block_size, num_tokens, max_blocks, rows=None, pad_len=1, scratch_block=-1, out=None):
     """One launch; every tensor int32 (other integers are converted)."""
     B, n_ids, i32 = q_lens.numel(), block_ids.numel(), torch.int32
     rows = ref._step_sizes(B, block_size, num_tokens, max_blocks, rows, pad_len, scratch_block)
     if seq_lens.numel() != B or block_offsets.numel() != B + 1:
         raise ValueError("step_tables: one length per sequence and one offset more")
-    if rows > 12000:
-        raise ValueError("step_tables: at most 12000 rows")
+    if rows > STEP_ROWS:
+        raise ValueError(f"step_tables: at most {STEP_ROWS} rows")
     _same_device(q_lens, seq_lens, block_ids, block_offsets)
     if not (q_lens.dtype == seq_lens.dtype == block_ids.dtype == block_offsets.dtype == i32 and q_lens.is_contiguous() and seq_lens.is_contiguous()
             and block_ids.is_contiguous() and block_offsets.is_contiguous()):

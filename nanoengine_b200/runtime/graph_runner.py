@@ -21,6 +21,8 @@ from typing import Dict, List
 
 import torch
 
+from .. import ops
+from ..ops.reference import StepTables
 from .context import ForwardContext
 
 
@@ -61,7 +63,11 @@ class DecodeGraphRunner:
         self.slot_mapping = torch.zeros(n, dtype=torch.long, device=dev)
         self.context_lens = torch.ones(self.max_bs, dtype=torch.int32, device=dev)
         self.block_tables = torch.zeros(self.max_bs, self.max_blocks, dtype=torch.int32, device=dev)
+        # models with positions on several axes read these instead
+        self.axes = torch.zeros(len(runner.position_axes), n, dtype=torch.long, device=dev) if runner.position_axes else None
         self.cu_seqlens_q = (torch.arange(self.max_bs + 1, dtype=torch.int32, device=dev) * q_len)
+        self.tables = StepTables(self.cu_seqlens_q, self.context_lens, self.positions, self.slot_mapping, self.block_tables,
+                                 torch.zeros(self.max_bs, dtype=torch.int32, device=dev))
         # recurrent-state models: slot of every row (padding rows and capture warm-ups use the scratch slot)
         self.gdn = runner.plan.gdn
         self.state_slots = torch.full((self.max_bs,), runner.cache.scratch_slot, dtype=torch.int32, device=dev)
@@ -98,11 +104,19 @@ class DecodeGraphRunner:
         n, q = ctx.num_seqs, self.q_len
         sb = self.r.cache.scratch_block
         self.input_ids[: n * q].copy_(ids)
-        self.positions[: n * q].copy_(pos)
-        self.slot_mapping[: n * q].copy_(ctx.slot_mapping)
-        self.context_lens[:n].copy_(ctx.context_lens)
         w = ctx.block_tables.shape[1]
-        self.block_tables[:n, :w].copy_(ctx.block_tables)
+        made_of = ctx.extras.get("tables_of")
+        if made_of is not None:
+            # straight into the captured buffers, padding rows included (their one page is the scratch page)
+            ops.step_tables(*made_of, b * q, max(w, -(-q // made_of[-1])), rows=b, pad_len=q, scratch_block=sb, out=self.tables)
+        else:
+            self.positions[: n * q].copy_(pos if self.axes is None else pos[0])
+            self.slot_mapping[: n * q].copy_(ctx.slot_mapping)
+            self.context_lens[:n].copy_(ctx.context_lens)
+            self.block_tables[:n, :w].copy_(ctx.block_tables)
+        if self.axes is not None:
+            self.axes[:, : n * q].copy_(pos)
+            self.axes[:, n * q: b * q].zero_()
         if self.gdn:
             self.state_slots[:n].copy_(ctx.state_slots)
             self.seq_fresh[:n].copy_(ctx.seq_fresh)
@@ -113,6 +127,7 @@ class DecodeGraphRunner:
         if n < b:
             # padding rows: q_len tokens of a one-page sequence on the scratch page
             self.input_ids[n * q: b * q].zero_()
+        if n < b and made_of is None:
             self.positions[n * q: b * q].copy_(torch.arange(q, device=ids.device).repeat(b - n))
             self.slot_mapping[n * q: b * q].copy_(sb * self.r.plan.block_size + torch.arange(q, device=ids.device).repeat(b - n))
             self.context_lens[n:b].fill_(q)
@@ -121,7 +136,7 @@ class DecodeGraphRunner:
     def _capture(self, b: int):
         sctx = self._static_ctx(b)
         q = self.q_len
-        ids, pos = self.input_ids[: b * q], self.positions[: b * q]
+        ids, pos = self.input_ids[: b * q], self.positions[: b * q] if self.axes is None else self.axes[:, : b * q]
         if self.gdn:
             # the warm-up runs execute real steps: point every row at the scratch slot so no live sequence's state advances
             # (rows sharing one slot race on it, which is harmless for scratch data); run() refills the live slots afterwards

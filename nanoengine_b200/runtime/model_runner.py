@@ -22,6 +22,8 @@ from ..config import Config
 from ..models.registry import get_model_class
 from ..models.weights import expert_owner_filter, iterate_safetensors, random_hf_weights
 from ..parallel.dist import DistContext, ParallelSpec, get_dist_context, init_dist_context
+from .. import ops
+from ..ops.reference import StepTables
 from .cache import KVCache, kv_budget_blocks, make_cache_plan, torch_dtype
 from .context import ForwardContext
 from .sampler import Sampler
@@ -82,6 +84,8 @@ class ModelRunner:
         self.graphs = None
         self.mtp_runner = None
         self._profiler = None
+        self.position_axes = self.mc.position_axes
+        self._image_axes = {}      # sequence id -> (positions [axes, prompt tokens], shift of what follows) of sequences with images
         self.h2d_bytes = 0          # bytes copied host -> device for step inputs (benchmark bookkeeping)
         self.d2h_bytes = 0          # bytes read back (sampled tokens, log-probabilities)
         self._last_decode = None
@@ -313,23 +317,55 @@ class ModelRunner:
             return t.pin_memory().to(self.device, non_blocking=True)
         return t
 
+    def _step_inputs(self, b, block_size: int):
+        """(host facts, token ids, tables, what `step_tables` made them of or None) of a step.  On a GPU the lengths, page lists and tokens travel in
+        one copy and the tables are built there; a step whose tokens do not stand where its lengths put them brings its tables from the host."""
+        if self.device.type == "cuda":
+            from ..ops import sm100
+            d = b.pack(block_size)
+            if d["consecutive"] and b.num_seqs <= sm100.STEP_ROWS:
+                n, ids = b.num_seqs, d["num_ids"]
+                q, seq, off, pages, tokens = self._to_dev(d["packed"]).split([n, n, n + 1, ids, d["packed"].shape[0] - 3 * n - 1 - ids])
+                made_of = (q, seq, pages, off, block_size)
+                return d, tokens.long(), ops.step_tables(*made_of, tokens.shape[0], d["max_blocks"]), made_of
+        d = b.prepare(block_size, 0)
+        t = StepTables(self._to_dev(d["cu_seqlens_q"]), self._to_dev(d["context_lens"]), self._to_dev(d["positions"]).long(),
+                       self._to_dev(d["slot_mapping"]), self._to_dev(d["block_tables"]).view(b.num_seqs, -1), self._to_dev(d["last_token_indices"]))
+        return d, self._to_dev(d["input_ids"]).long(), t, None
+
+    def _axis_positions(self, b, positions: torch.Tensor) -> torch.Tensor:
+        """Positions [axes, T] of a model that has several: those of a text token are alike on all of them, a sequence with images brings its own."""
+        A = len(self.position_axes)
+        if not any(int(s) in self._image_axes for s in b.seq_ids):
+            return positions.expand(A, -1).contiguous()
+        out = np.tile(np.asarray(b.positions, dtype=np.int64), (A, 1))
+        lo = 0
+        for sid, q in zip(b.seq_ids, b.q_lens):
+            own = self._image_axes.get(int(sid))
+            if own is not None:
+                prompt, shift = own
+                at = out[0, lo: lo + q].copy()
+                out[:, lo: lo + q] = np.where(at < prompt.shape[1], prompt[:, np.minimum(at, prompt.shape[1] - 1)], at + shift)
+            lo += q
+        return self._to_dev(out)
+
     def prepare(self, b) -> ForwardContext:
         bs = self.plan.block_size
         if b.is_dummy or b.num_seqs == 0:
             return self._dummy_context(b.is_prefill)
-        d = b.prepare(bs, 0)
+        d, ids, t, made_of = self._step_inputs(b, bs)
         q_lens = b.q_lens
         uniform = q_lens[0] if all(q == q_lens[0] for q in q_lens) else 0
         ctx = ForwardContext(
-            is_prefill=b.is_prefill, num_seqs=b.num_seqs, num_tokens=len(b.input_ids),
-            cu_seqlens_q=self._to_dev(d["cu_seqlens_q"]), context_lens=self._to_dev(d["context_lens"]),
-            slot_mapping=self._to_dev(d["slot_mapping"]), block_tables=self._to_dev(d["block_tables"]).view(b.num_seqs, -1),
+            is_prefill=b.is_prefill, num_seqs=b.num_seqs, num_tokens=ids.shape[0],
+            cu_seqlens_q=t.cu_seqlens_q, context_lens=t.context_lens, slot_mapping=t.slot_mapping, block_tables=t.block_tables,
             max_seqlen_q=int(d["max_seqlen_q"]), max_seqlen_k=int(d["max_seqlen_k"]),
-            last_token_indices=self._to_dev(d["last_token_indices"]), q_len_uniform=uniform,
+            last_token_indices=t.last_token_indices, q_len_uniform=uniform,
             kv_caches=self.cache.layers, indexer_caches=self.cache.indexer_layers,
             cu_seqlens_q_host=d["cu_seqlens_q"].tolist(), context_lens_host=d["context_lens"].tolist())
-        ctx.extras["input_ids"] = self._to_dev(d["input_ids"]).long()
-        ctx.extras["positions"] = self._to_dev(d["positions"]).long()
+        ctx.extras["input_ids"] = ids
+        ctx.extras["positions"] = t.positions if self.position_axes is None else self._axis_positions(b, t.positions)
+        ctx.extras["tables_of"] = made_of
         # every sequence of the step brings its whole context with it (no cached prefix, no earlier chunk)
         ctx.extras["no_prefix"] = bool(b.is_prefill and all(int(n) == int(q) for n, q in zip(b.seq_lens, q_lens)))
         if self.cache.hisparse is not None:
@@ -361,7 +397,7 @@ class ModelRunner:
             last_token_indices=torch.tensor([0], dtype=torch.int32, device=dev), q_len_uniform=1, is_dummy=True,
             kv_caches=self.cache.layers, indexer_caches=self.cache.indexer_layers, cu_seqlens_q_host=[0, 1], context_lens_host=[1])
         ctx.extras["input_ids"] = torch.zeros(1, dtype=torch.long, device=dev)
-        ctx.extras["positions"] = torch.zeros(1, dtype=torch.long, device=dev)
+        ctx.extras["positions"] = torch.zeros(1 if self.position_axes is None else (len(self.position_axes), 1), dtype=torch.long, device=dev)
         if self.cache.hisparse is not None:
             ctx.hisparse = self.cache.hisparse
             ctx.hs_slots = torch.tensor([self.cache.hisparse.scratch_slot], dtype=torch.int32, device=dev)
@@ -377,10 +413,11 @@ class ModelRunner:
     # ---- execution -----------------------------------------------------------------------------
     # ---- vision embeddings -----------------------------------------------------------------------
     def register_vision(self, seq_id: int, prompt_token_ids, image_token_id: int, embeddings=None, pool_desc=None, slot: int = -1,
-                        num_tokens: int = 0) -> int:
+                        num_tokens: int = 0, grid_thw=None, merge: int = 2) -> int:
         """Attach the image embeddings of a request: the rows replace, in order, the embeddings of its `image_token_id`
         prompt tokens during prefill (also when the prompt is prefetched in chunks).  `embeddings` [n, hidden] directly, or
-        a pool descriptor of a vision encoder (`vl.EmbeddingPool.export`) plus the slot to read.
+        a pool descriptor of a vision encoder (`vl.EmbeddingPool.export`) plus the slot to read.  With `grid_thw` a model whose rotary positions
+        have several axes places the image tokens by time, row and column until the request is released.
         Parity: reference runtime/runner/vision_embed.py:33-82 (masked scatter of image rows), :84-140 (one-sided fetch)."""
         if embeddings is None:
             from ..vl.embedding_pool import EmbeddingReader
@@ -395,12 +432,16 @@ class ModelRunner:
             raise ValueError(f"request {seq_id}: {int(is_img.sum())} image tokens in the prompt but {embeddings.shape[0]} embedding rows")
         if embeddings.shape[1] != self.mc.hidden_size:
             raise ValueError("embedding width differs from the model's hidden size")
+        if grid_thw and self.position_axes is not None:
+            from ..vl.positions import image_positions
+            self._image_axes[int(seq_id)] = image_positions(is_img, grid_thw, merge)
         self.__dict__.setdefault("_vision", {})[int(seq_id)] = (np.concatenate([[0], np.cumsum(is_img)]), is_img,
                                                                   embeddings.to(self.device, self.dtype))
         return embeddings.shape[0]
 
     def release_vision(self, seq_id: int) -> None:
         self.__dict__.get("_vision", {}).pop(int(seq_id), None)
+        self._image_axes.pop(int(seq_id), None)
 
     def _vision_inputs_embeds(self, b, ctx: ForwardContext):
         """inputs_embeds of a prefill step when one of its sequences carries image embeddings, else None."""

@@ -3,6 +3,7 @@ Parity: reference dlengine/vl/ (vision/encoder.py, encoder/encoder_engine.py, se
 runtime/context/cache/emb.py."""
 from .embedding_pool import EmbeddingPool
 from .encoder_engine import EncoderConfig, EncoderEngine
+from .positions import image_positions
 from .vision import VisionConfig, VisionModel
 
-__all__ = ["EmbeddingPool", "EncoderConfig", "EncoderEngine", "VisionConfig", "VisionModel"]
+__all__ = ["EmbeddingPool", "EncoderConfig", "EncoderEngine", "VisionConfig", "VisionModel", "image_positions"]

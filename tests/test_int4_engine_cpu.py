@@ -122,3 +122,77 @@ def test_refusals():
     assert Config(model="tiny", model_config=tiny_qwen3(head_dim=64), dummy_weight=True, device="cuda", kv_cache_dtype="int4").kvcache_block_size == 64
     with pytest.raises(ValueError, match="int4"):
         Config(model="tiny", model_config=tiny_qwen3(), dummy_weight=True, device="cpu", kv_cache_dtype="int8")
+
+
+# ---- image tokens at a time, a row and a column ----------------------------------------------------
+IMG = 7
+GRIDS = [(1, 4, 6), (2, 2, 4)]                       # patches: 2 x 3 and 2 x (1 x 2) tokens
+PROMPT = [3, 11] + [IMG] * 6 + [25, 99, 14] + [IMG] * 4 + list(range(30, 50))
+
+
+def expected_positions(tokens):
+    out, p, i, images = [], 0, 0, [(t, h // 2, w // 2) for t, h, w in GRIDS]
+    while i < tokens:
+        if i < len(PROMPT) and PROMPT[i] == IMG:
+            t, h, w = images.pop(0)
+            out += [(p + a, p + b, p + c) for a in range(t) for b in range(h) for c in range(w)]
+            i, p = i + t * h * w, p + max(t, h, w)
+        else:
+            out.append((p, p, p))
+            i, p = i + 1, p + 1
+    return torch.tensor(out).t()
+
+
+@pytest.mark.parametrize("kv", ["float32", "int4"])
+@pytest.mark.parametrize("kw", [{}, dict(max_num_batched_tokens=16)])
+def test_image_tokens_stand_at_time_row_and_column(kv, kw):
+    sp = SamplingParams(temperature=0.0, max_tokens=5, ignore_eos=True)
+    emb = torch.randn(10, 128, generator=torch.Generator().manual_seed(1)) * 0.02
+    seen, text, got = {}, {}, {}
+    for grids in (GRIDS, None):
+        llm = make("qwen3", kv, enable_prefix_caching=False, model_config=tiny_qwen3(mrope_section=[6, 5, 5], mrope_interleaved=True), **kw)
+        runner = llm.engine.executor.runner
+        plain = runner.prepare
+
+        def prepare(b, seen=seen, text=text, grids=grids, plain=plain):
+            ctx = plain(b)
+            lo = 0
+            for sid, q, n in zip(b.seq_ids, b.q_lens, b.seq_lens):
+                pos = ctx.extras["positions"][:, lo: lo + q]
+                (seen if int(sid) == 1 and grids else text).setdefault(int(sid), {})[int(n) - q] = pos.clone()
+                lo += q
+            return ctx
+
+        runner.prepare = prepare
+        llm.engine.add_vision_request(PROMPT, IMG, embeddings=emb, sampling_params=sp, seq_id=1, grid_thw=grids)
+        llm.engine.add_request(list(range(60, 90)), sp, seq_id=2)
+        got[bool(grids)] = {o["seq_id"]: o["token_ids"] for o in llm.generate()}
+        assert not runner._image_axes and not llm.engine._with_axes                # given back when the request is through
+    whole = torch.cat([seen[1][k] for k in sorted(seen[1])], 1)
+    assert torch.equal(whole, expected_positions(len(PROMPT) + 4))
+    for parts in text.values():                                                     # tokens without grids: their index on every axis
+        flat = torch.cat([parts[k] for k in sorted(parts)], 1)
+        assert torch.equal(flat, torch.arange(flat.shape[1]).expand(3, -1))
+    assert got[True][2] == got[False][2]
+    if not kw:
+        # one step over everything gives the tokens that the cached steps gave
+        runner.prepare = plain
+        llm = make("qwen3", kv, enable_prefix_caching=False, model_config=tiny_qwen3(mrope_section=[6, 5, 5], mrope_interleaved=True), max_num_batched_tokens=16)
+        llm.engine.add_vision_request(PROMPT, IMG, embeddings=emb, sampling_params=sp, seq_id=1, grid_thw=GRIDS)
+        assert llm.generate()[0]["token_ids"] == got[True][1]
+
+
+def test_image_grids_that_do_not_fit_are_refused():
+    mc = tiny_qwen3(mrope_section=[6, 5, 5])
+    emb = torch.zeros(10, 128)
+    llm = make("qwen3", "int4", model_config=mc)
+    for grids in ([(1, 4, 6)], [(1, 4, 6), (2, 2, 6)], [(1, 3, 6), (2, 2, 4)], GRIDS + [(1, 2, 2)]):
+        with pytest.raises(ValueError):
+            llm.engine.add_vision_request(PROMPT, IMG, embeddings=emb, sampling_params=SP, grid_thw=grids)
+    assert not llm.engine.executor.runner._image_axes and not llm.engine._with_axes
+    seq = llm.engine.add_vision_request(PROMPT, IMG, embeddings=emb, sampling_params=SP, grid_thw=GRIDS)
+    assert llm.engine.abort(seq) and not llm.engine.executor.runner._image_axes
+    with pytest.raises(ValueError, match="mrope_section"):
+        make("qwen3", "int4", model_config=tiny_qwen3(mrope_section=[8, 5, 5]))
+    got = ModelConfig.from_dict({"architectures": ["Qwen3ForCausalLM"], "head_dim": 32, "rope_scaling": {"mrope_section": [6, 5, 5], "mrope_interleaved": True}})
+    assert got.position_axes == [6, 5, 5] and got.mrope_interleaved
