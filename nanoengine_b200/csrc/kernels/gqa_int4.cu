@@ -2,22 +2,29 @@
 //
 //   softmax(q k^T scale) v with k = (c - 8) s of 4-bit codes, a scale per 32 dims; causal, optionally the last `window` keys only
 //
-// Bound by HBM: D/2 + D/32 bytes a key row, 17/64 of bf16.  A unit of work is a tile of 64 keys (32 for heads of 256) for up to 16 (token, head of the
+// Least traffic: D/2 + D/32 bytes a key row, 17/64 of bf16.  A unit of work is a tile of 64 keys (32 for heads of 256) for up to 16 (token, head of the
 // group) rows of one sequence and KV head.  The units of the whole batch, laid end to end, are cut into equal shares, one per warp that fits the GPU:
 // ragged contexts keep no SM waiting, whatever their number, and no warp waits for another.  A warp walks its share with a ring of bulk copies of its own.
 // Where a share cuts a row tile, the pieces are written as 32-bit partial results, two places per warp, and a second kernel joins the pieces of every
 // tile that a cut runs through.
 //
 // A key is unpacked once, in registers, straight into the fragments of mma.m16n8k16: a lane owns a contiguous quarter of a key row and an eighth of a value
-// row; the dims of a step of the first product and the keys of a step of the second are permuted to match (query rows and probabilities follow).  tcgen05
-// would want the unpacked tile in shared memory: 16 rows fill an eighth of its M = 128, and the 32 KB of bf16 that a tile of 64 keys becomes would cross
-// shared memory twice, which takes longer than its 8.5 KB take to come from HBM.  Portions with many rows per key run on the tensor-core prompt kernel over
-// expanded pages instead.
+// row; the dims of a step of the first product and the keys of a step of the second are permuted to match (query rows and probabilities follow).  Up to 16
+// rows of queries are the 16 rows of a product.  Where a sequence has no more than 8, the products are transposed (S^T = K Q^T, O^T = V^T P^T): keys and value
+// dims are the 16 rows, the same unpacked registers make half as many products, and the results take half the registers, so that a third CTA fits an SM.
+// Portions with many rows per key run on the tensor-core prompt kernel over expanded pages instead.
 //
 // A masked nibble is a bf16 pair of subnormals c 2^-133 (16 c 2^-133 for the upper nibble of a byte), so that one fused multiply-add per pair gives
 // (c - 8) s 2^-24, exactly; the 2^24 goes into the softmax scale and the last division.  Scores, maxima, sums and results are 32-bit, probabilities enter
-// the second product as bf16 (2^-9 each) and their sum is a column of ones of the same product.  Every byte stands for a finite value, so a masked key
+// the second product as bf16 (2^-9 each) and their sum is a column (row) of ones of the same product.  Every byte stands for a finite value, so a masked key
 // (probability 0) adds nothing whatever its page holds.
+//
+// Bound by the unpacking and the products, not by HBM (cycles of a warp for a tile of 64 keys, 16 rows, two warps a scheduler: waiting for copies 290, scores 1460,
+// maximum 290, values 1770, next copy 580; a product and the two pairs that feed it take 9.7 cycles of their pipes).  Measured (B200, us, GB/s of 6530): 128 x 4096
+// keys, 64 / 4 heads of 128 (16 rows): 89, 3210; 32 / 8 heads (4 rows): 116, 4920; 2 x 131072 keys, 64 / 4: 53; 60 x 3000, 16 / 2 heads of 256: 42; 33 x 2504, four tokens,
+// 32 / 8: 42; 1 x 1001: 10.  Slower: queries in shared memory, tiles of 32 keys, copies by cp.async, three CTAs per SM with 16 rows (they spill).  tcgen05 with the keys
+// unpacked into tensor memory and the values into shared memory, three CTAs per SM, a warp of its own for copies and products: 116 where this one takes 89; the
+// unpacked values cross shared memory twice, and barriers between unpacking, products and softmax leave the pipes idle.
 #include "kv4.cuh"
 
 namespace ne {
@@ -30,25 +37,25 @@ struct I4Args {
   const uint8_t* k; const uint8_t* v; int num_blocks, block_size;
   const int* block_tables; long long bt_ld; int bt_width;
   const int* cu_seqlens_q; const int* context_lens; int num_seqs;
-  int T, Hq, Hkv, g, tq, head_tiles, window, shares;   // tq tokens x min(g, 16) heads a row tile; head_tiles = ceil(g / 16)
+  int T, Hq, Hkv, g, rows, tq, head_tiles, window, shares;   // rows of a row tile: tq tokens x min(g, rows) heads; head_tiles = ceil(g / rows)
   int max_tiles;                                       // places in cuts
   float scale_log2;
   __nv_bfloat16* out;                                  // [T, Hq, D]
-  float* part; float* lse2;                            // [shares, 2, 16, D], [shares, 2, 16]
+  float* part; float* lse2;                            // [shares, 2, rows, D], [shares, 2, rows]
   int4* cuts;                                          // [1 + row tiles]: how many row tiles there are; what the join needs of each
 };
 
-template <int D> struct I4Geo {
+template <int D, int R> struct I4Geo {                                  // R: rows of a row tile, 8 or 16
   static constexpr int keys = D == 256 ? 32 : 64;                       // of a tile
-  static constexpr int slots = D == 256 ? 2 : 3;                        // of a warp's ring
-  static constexpr int ctas = D == 64 ? 3 : 2;                          // resident per SM
+  static constexpr int slots = D == 256 || (D == 128 && R == 8) ? 2 : 3;   // of a warp's ring
+  static constexpr int ctas = D == 64 || (D == 128 && R == 8) ? 3 : 2;  // resident per SM
   static constexpr int row = D / 2, srow = D / 32;                      // bytes of a row's codes and scales
   static constexpr int codes = keys * row, half = codes + keys * srow, stage = 2 * half;
   static constexpr int words = D / 32;                                  // words of a key row a lane owns (a quarter of the row)
   static constexpr int vwords = D / 64;                                 // words of a value row a lane owns (an eighth)
   static constexpr int ks = D / 16;                                     // k steps of the first product
   static constexpr int nt = D / 8;                                      // column tiles of the second one
-  static constexpr bool q_regs = D <= 128;                              // query fragments in registers, else in shared memory
+  static constexpr bool q_regs = D <= 128 || R == 8;                            // query fragments in registers, else in shared memory
   static constexpr int warp_bytes = slots * stage + (q_regs ? 0 : ks * 512);
   static constexpr int smem = kI4Warps * warp_bytes;
 };
@@ -146,8 +153,8 @@ struct I4Piece {
 };
 template <int KEYS> __device__ __forceinline__ void i4_fill(const I4Args& a, I4Piece& p, int left) {
   p.units = min(p.s.per_tile - p.unit, left);
-  p.gh = min(a.g - p.ht * 16, 16);
-  p.head0 = p.hkv * a.g + p.ht * 16;
+  p.gh = min(a.g - p.ht * a.rows, a.rows);
+  p.head0 = p.hkv * a.g + p.ht * a.rows;
   p.tok0 = p.s.q_beg + p.tile * a.tq;
   p.n_tok = p.tok0 < 0 ? 0 : min(min(a.tq, p.s.q_len - p.tile * a.tq), a.T - p.tok0);
   p.base_limit = p.s.ctx - p.s.q_len + p.tile * a.tq;                    // last key the tile's first token sees
@@ -198,6 +205,13 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Element pairs of an 8 x 8 matrix of 16-bit values, lane 4 i + j with (i, 2 j) and (i, 2 j + 1), to those of its transpose
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
 // Multipliers of one scale (or of a pair of scales) as bf16 pairs, from (byte << 4) in both halves: s 2^109 for the lower nibble of a byte, s 2^105 for the
 // upper one, -8 s 2^-24.  None leaves bf16's exponents.  (Two of them by exact products: the integer pipe is the busier one.)
 struct I4Scale { uint32_t lo, hi, z; };
@@ -208,9 +222,10 @@ __device__ __forceinline__ I4Scale i4_scale(uint32_t b4) {
 __device__ __forceinline__ uint32_t i4_lower(uint32_t w, const I4Scale& s) { return hfma2_bf16(w & 0x000F000Fu, s.lo, s.z); }
 __device__ __forceinline__ uint32_t i4_upper(uint32_t w, const I4Scale& s) { return hfma2_bf16(w & 0x00F000F0u, s.hi, s.z); }
 
-template <int D, bool kPlain>
-__global__ void __launch_bounds__(kI4Threads, I4Geo<D>::ctas) gqa_int4_kernel(const I4Args a) {
-  using G = I4Geo<D>;
+template <int D, int R, bool kPlain>
+__global__ void __launch_bounds__(kI4Threads, I4Geo<D, R>::ctas) gqa_int4_kernel(const I4Args a) {
+  using G = I4Geo<D, R>;
+  constexpr bool kNarrow = R == 8;                                       // the keys and the value dims are the 16 rows of a product, the query rows its 8 columns
   constexpr int ST = G::slots, JT = G::keys / 8;                         // JT: column tiles of the scores
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ I4Shared sh;
@@ -301,21 +316,30 @@ __global__ void __launch_bounds__(kI4Threads, I4Geo<D>::ctas) gqa_int4_kernel(co
     int id = page_of(p, p.t_begin + ST);
 
     // this lane's two query rows (fragment rows n and n + 8): token and head
-    const int t0 = gh == 16 ? 0 : n / gh, t1 = gh == 16 ? 0 : (n + 8) / gh, h0 = n - t0 * gh, h1 = n + 8 - t1 * gh;
+    // (narrow: it loads row n and has results of rows 2 c and 2 c + 1)
+    const int r0 = kNarrow ? 2 * c : n, r1 = kNarrow ? 2 * c + 1 : n + 8;
+    const int t0 = r0 / gh, t1 = r1 / gh, h0 = r0 - t0 * gh, h1 = r1 - t1 * gh;
     const bool ok0 = t0 < n_tok, ok1 = t1 < n_tok;
     const int lim0 = ok0 ? base_limit + t0 : -1, lim1 = ok1 ? base_limit + t1 : -1;
-    uint32_t qa[G::q_regs ? G::ks : 1][4];
+    constexpr int QF = kNarrow ? 2 : 4;                                  // registers of a query fragment
+    uint32_t qa[G::q_regs ? G::ks : 1][QF];
     uint4* sq = reinterpret_cast<uint4*>(ring + ST * G::stage);
     {
-      const uint2* p0 = reinterpret_cast<const uint2*>(a.q + (long long)(tok0 + (ok0 ? t0 : 0)) * a.q_ld + (long long)(head0 + h0) * D + c * (D / 4));
-      const uint2* p1 = reinterpret_cast<const uint2*>(a.q + (long long)(tok0 + (ok1 ? t1 : 0)) * a.q_ld + (long long)(head0 + h1) * D + c * (D / 4));
+      const int tq0 = kNarrow ? n / gh : t0, hq0 = kNarrow ? n - tq0 * gh : h0;
+      const bool okq = kNarrow ? tq0 < n_tok : ok0;
+      const uint2* p0 = reinterpret_cast<const uint2*>(a.q + (long long)(tok0 + (okq ? tq0 : 0)) * a.q_ld + (long long)(head0 + (okq ? hq0 : 0)) * D + c * (D / 4));
+      const uint2* p1 = reinterpret_cast<const uint2*>(a.q + (long long)(tok0 + (ok1 ? t1 : 0)) * a.q_ld + (long long)(head0 + (ok1 ? h1 : 0)) * D + c * (D / 4));
       if constexpr (G::q_regs) {
-        // the products want the four words of a step in neighbouring registers, the loads pairs of them: without an operation in between, every product moves them
+        // the products want the words of a step in neighbouring registers, the loads pairs of them: without an operation in between, every product moves them
         const uint32_t nil = (uint32_t)a.shares >> 31;
 #pragma unroll
         for (int ks = 0; ks < G::ks; ks++) {
-          const uint2 x0 = ok0 ? p0[ks] : make_uint2(0, 0), x1 = ok1 ? p1[ks] : make_uint2(0, 0);
-          qa[ks][0] = x0.x ^ nil; qa[ks][1] = x1.x ^ nil; qa[ks][2] = x0.y ^ nil; qa[ks][3] = x1.y ^ nil;
+          const uint2 x0 = okq ? p0[ks] : make_uint2(0, 0);
+          if constexpr (kNarrow) { qa[ks][0] = x0.x ^ nil; qa[ks][1] = x0.y ^ nil; }
+          else {
+            const uint2 x1 = ok1 ? p1[ks] : make_uint2(0, 0);
+            qa[ks][0] = x0.x ^ nil; qa[ks][1] = x1.x ^ nil; qa[ks][2] = x0.y ^ nil; qa[ks][3] = x1.y ^ nil;
+          }
         }
       } else {
 #pragma unroll
@@ -327,9 +351,10 @@ __global__ void __launch_bounds__(kI4Threads, I4Geo<D>::ctas) gqa_int4_kernel(co
       }
     }
 
-    float o[G::nt][4], l[4] = {0.f, 0.f, 0.f, 0.f};
+    constexpr int NT = kNarrow ? G::nt / 2 : G::nt, SJ = kNarrow ? JT / 2 : JT;        // products' results: columns or (narrow) pairs of rows of D and of a tile of keys
+    float o[NT][4], l[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < G::nt; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    for (int i = 0; i < NT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY;
 
 #pragma unroll 1
@@ -353,9 +378,10 @@ __global__ void __launch_bounds__(kI4Threads, I4Geo<D>::ctas) gqa_int4_kernel(co
         __syncwarp();
       }
         // scores: column tile j = (kk, t) holds in fragment column 2 c' + e the key 16 kk + 4 (2 t + e) + (c' ^ e): neighbouring lanes read neighbouring rows
-        float s[JT][4];
+        // (narrow: fragment row n of the pair (kk, 0), (kk, 1) is the key of column n)
+        float s[SJ][4];
 #pragma unroll
-        for (int j = 0; j < JT; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+        for (int j = 0; j < SJ; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
 #pragma unroll
         for (int jb = 0; jb < JT; jb += 2) {
 #pragma unroll
@@ -373,6 +399,13 @@ __global__ void __launch_bounds__(kI4Threads, I4Geo<D>::ctas) gqa_int4_kernel(co
             }
 #pragma unroll
             for (int i = 0; i < NW; i++) {
+              if constexpr (kNarrow) {
+                const uint32_t (&qe)[2] = qa[2 * (i0 + i)], (&qo)[2] = qa[2 * (i0 + i) + 1];
+                const uint32_t ke[4] = {i4_lower(w[0][i], sc[0]), i4_lower(w[1][i], sc[1]), i4_upper(w[0][i], sc[0]), i4_upper(w[1][i], sc[1])};
+                mma_16816(s[jb / 2], ke, qe[0], qe[1]);
+                const uint32_t ko[4] = {i4_lower(w[0][i] >> 8, sc[0]), i4_lower(w[1][i] >> 8, sc[1]), i4_upper(w[0][i] >> 8, sc[0]), i4_upper(w[1][i] >> 8, sc[1])};
+                mma_16816(s[jb / 2], ko, qo[0], qo[1]);
+              } else {
               uint32_t qe[4], qo[4];
               if constexpr (G::q_regs) {
 #pragma unroll
@@ -386,6 +419,7 @@ __global__ void __launch_bounds__(kI4Threads, I4Geo<D>::ctas) gqa_int4_kernel(co
               for (int j = 0; j < 2; j++) mma_16816(s[jb + j], qe, i4_lower(w[j][i], sc[j]), i4_upper(w[j][i], sc[j]));
 #pragma unroll
               for (int j = 0; j < 2; j++) mma_16816(s[jb + j], qo, i4_lower(w[j][i] >> 8, sc[j]), i4_upper(w[j][i] >> 8, sc[j]));
+              }
             }
           }
         }
@@ -396,43 +430,57 @@ __global__ void __launch_bounds__(kI4Threads, I4Geo<D>::ctas) gqa_int4_kernel(co
           for (int j = 0; j < JT; j++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              const int key = key0 + 16 * (j >> 1) + 4 * (2 * (j & 1) + e) + (c ^ e);
-              if (key > lim0 || key <= low0) s[j][e] = -INFINITY;
-              if (key > lim1 || key <= low1) s[j][2 + e] = -INFINITY;
+              // narrow: tile j's half of the pair's results, one key for both rows
+              const int key = key0 + 16 * (j >> 1) + (kNarrow ? 4 * (2 * (j & 1) + (n & 1)) + ((n >> 1) ^ (n & 1)) : 4 * (2 * (j & 1) + e) + (c ^ e));
+              float& y0 = kNarrow ? s[j / 2][2 * (j & 1)] : s[kNarrow ? 0 : j][e];
+              float& y1 = kNarrow ? s[j / 2][2 * (j & 1) + 1] : s[kNarrow ? 0 : j][2 + e];
+              if (key > lim0 || key <= low0) y0 = -INFINITY;
+              if (key > lim1 || key <= low1) y1 = -INFINITY;
             }
         }
         float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < JT; j++) {
-          x0 = fmaxf(x0, fmaxf(s[j][0], s[j][1]));
-          x1 = fmaxf(x1, fmaxf(s[j][2], s[j][3]));
+        for (int j = 0; j < SJ; j++) {
+          x0 = fmaxf(x0, fmaxf(s[j][0], s[j][kNarrow ? 2 : 1]));
+          x1 = fmaxf(x1, fmaxf(s[j][kNarrow ? 1 : 2], s[j][3]));
         }
         x0 *= scale; x1 *= scale;
         // the reference maximum moves only when a score exceeds it by more than 2^8 (or is the first): rare, so that the rows' lanes compare notes only then
         if (__any_sync(0xffffffffu, x0 > m0 + 8.f || x1 > m1 + 8.f || (m0 == -INFINITY && x0 > m0) || (m1 == -INFINITY && x1 > m1))) {
 #pragma unroll
-          for (int d = 1; d < 4; d <<= 1) {
+          for (int d = kNarrow ? 4 : 1; d < (kNarrow ? 32 : 4); d <<= 1) {
             x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
             x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
           }
           const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
           const float f0 = n0 == -INFINITY ? 1.f : exp2f(m0 - n0), f1 = n1 == -INFINITY ? 1.f : exp2f(m1 - n1);
           m0 = n0; m1 = n1;
-          l[0] *= f0; l[1] *= f0; l[2] *= f1; l[3] *= f1;
+          // narrow: columns 2 c and 2 c + 1 alternate
+          const float fa = kNarrow ? f1 : f0, fb = kNarrow ? f0 : f1;
+          l[0] *= f0; l[1] *= fa; l[2] *= fb; l[3] *= f1;
 #pragma unroll
-          for (int i = 0; i < G::nt; i++) { o[i][0] *= f0; o[i][1] *= f0; o[i][2] *= f1; o[i][3] *= f1; }
+          for (int i = 0; i < NT; i++) { o[i][0] *= f0; o[i][1] *= fa; o[i][2] *= fb; o[i][3] *= f1; }
         }
         const float z0 = m0 == -INFINITY ? 0.f : -m0, z1 = m1 == -INFINITY ? 0.f : -m1;
 #pragma unroll
         for (int kk = 0; kk < G::keys / 16; kk++) {
           uint32_t pr[4];
+          if constexpr (kNarrow) {
+            // a lane has two rows of one key, the product wants two keys of one row
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+              pr[t] = transpose_8x8(pack_bf16x2(exp2f(fmaf(s[kk][2 * t], scale, z0)), exp2f(fmaf(s[kk][2 * t + 1], scale, z1))));
+            const uint32_t ones[4] = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+            mma_16816(l, ones, pr[0], pr[1]);                            // the sum of the probabilities as they are rounded
+          } else {
 #pragma unroll
           for (int t = 0; t < 2; t++) {
             const float (&v)[4] = s[2 * kk + t];
             pr[2 * t] = pack_bf16x2(exp2f(fmaf(v[0], scale, z0)), exp2f(fmaf(v[1], scale, z0)));
             pr[2 * t + 1] = pack_bf16x2(exp2f(fmaf(v[2], scale, z1)), exp2f(fmaf(v[3], scale, z1)));
           }
-          mma_16816(l, pr, 0x3F803F80u, 0x3F803F80u);                    // the sum of the probabilities as they are rounded
+          mma_16816(l, pr, 0x3F803F80u, 0x3F803F80u);
+          }
           // values: this lane's four keys of the step, an eighth of each row
           uint32_t w[4][G::vwords], sb[4];
 #pragma unroll
@@ -450,14 +498,14 @@ __global__ void __launch_bounds__(kI4Threads, I4Geo<D>::ctas) gqa_int4_kernel(co
             // a word's low half: even dims 0 2 4 6, high half: odd dims; two keys side by side
             const uint32_t al = __byte_perm(w[0][i], w[1][i], 0x5410), ah = __byte_perm(w[0][i], w[1][i], 0x7632);
             const uint32_t bl = __byte_perm(w[2][i], w[3][i], 0x5410), bh = __byte_perm(w[2][i], w[3][i], 0x7632);
-            mma_16816(o[8 * i + 0], pr, i4_lower(al, sa), i4_lower(bl, sz));
-            mma_16816(o[8 * i + 1], pr, i4_lower(ah, sa), i4_lower(bh, sz));
-            mma_16816(o[8 * i + 2], pr, i4_upper(al, sa), i4_upper(bl, sz));
-            mma_16816(o[8 * i + 3], pr, i4_upper(ah, sa), i4_upper(bh, sz));
-            mma_16816(o[8 * i + 4], pr, i4_lower(al >> 8, sa), i4_lower(bl >> 8, sz));
-            mma_16816(o[8 * i + 5], pr, i4_lower(ah >> 8, sa), i4_lower(bh >> 8, sz));
-            mma_16816(o[8 * i + 6], pr, i4_upper(al >> 8, sa), i4_upper(bl >> 8, sz));
-            mma_16816(o[8 * i + 7], pr, i4_upper(ah >> 8, sa), i4_upper(bh >> 8, sz));
+            auto both = [&](int j, uint32_t a0, uint32_t b0, uint32_t a1, uint32_t b1) {       // dims j and j + 1 of the lane's eight: first keys, second keys
+              if constexpr (kNarrow) { const uint32_t x[4] = {a0, a1, b0, b1}; mma_16816(o[4 * i + j / 2], x, pr[0], pr[1]); }
+              else { mma_16816(o[kNarrow ? 0 : 8 * i + j], pr, a0, b0); mma_16816(o[kNarrow ? 0 : 8 * i + j + 1], pr, a1, b1); }
+            };
+            both(0, i4_lower(al, sa), i4_lower(bl, sz), i4_lower(ah, sa), i4_lower(bh, sz));
+            both(2, i4_upper(al, sa), i4_upper(bl, sz), i4_upper(ah, sa), i4_upper(bh, sz));
+            both(4, i4_lower(al >> 8, sa), i4_lower(bl >> 8, sz), i4_lower(ah >> 8, sa), i4_lower(bh >> 8, sz));
+            both(6, i4_upper(al >> 8, sa), i4_upper(bl >> 8, sz), i4_upper(ah >> 8, sa), i4_upper(bh >> 8, sz));
           }
         }
         __syncwarp();                                                    // every lane has read the slot
@@ -480,27 +528,36 @@ __global__ void __launch_bounds__(kI4Threads, I4Geo<D>::ctas) gqa_int4_kernel(co
         if (p.t_begin + i < p.t_end) fetch(p, p.t_begin + i, slot + i < ST ? slot + i : slot + i - ST, page_of(p, p.t_begin + i));
     }
 
-    const float inv0 = l[0] == 0.f ? 0.f : 16777216.f / l[0], inv1 = l[2] == 0.f ? 0.f : 16777216.f / l[2];       // a NaN stays one
+    const float sum0 = l[0], sum1 = kNarrow ? l[1] : l[2];
+    const float inv0 = sum0 == 0.f ? 0.f : 16777216.f / sum0, inv1 = sum1 == 0.f ? 0.f : 16777216.f / sum1;       // a NaN stays one
     const long long row0 = (long long)(tok0 + t0) * a.Hq + head0 + h0, row1 = (long long)(tok0 + t1) * a.Hq + head0 + h1;
-    const long long at = ((long long)mine * 2 + (head ? 1 : 0)) * 16;    // a row tile's first piece: the share's second place
-#pragma unroll
-    for (int e = 0; e < 2; e++)
-#pragma unroll
-      for (int i = 0; i < G::nt / 4; i++) {                              // dims (2 c + e) D/8 + 4 i ..
-        const int d = (2 * c + e) * (D / 8) + 4 * i;
-        const float4 x = make_float4(o[4 * i][e] * inv0, o[4 * i + 1][e] * inv0, o[4 * i + 2][e] * inv0, o[4 * i + 3][e] * inv0);
-        const float4 y = make_float4(o[4 * i][2 + e] * inv1, o[4 * i + 1][2 + e] * inv1, o[4 * i + 2][2 + e] * inv1, o[4 * i + 3][2 + e] * inv1);
-        if (whole) {
-          if (ok0) *reinterpret_cast<uint2*>(a.out + row0 * D + d) = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
-          if (ok1) *reinterpret_cast<uint2*>(a.out + row1 * D + d) = make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
-        } else {
-          if (ok0) *reinterpret_cast<float4*>(a.part + (at + n) * D + d) = x;
-          if (ok1) *reinterpret_cast<float4*>(a.part + (at + n + 8) * D + d) = y;
-        }
+    const long long at = ((long long)mine * 2 + (head ? 1 : 0)) * R;     // a row tile's first piece: the share's second place
+    auto put = [&](int d, const float4& x, const float4& y) {             // dims d .. d + 3 of both rows
+      if (whole) {
+        if (ok0) *reinterpret_cast<uint2*>(a.out + row0 * D + d) = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
+        if (ok1) *reinterpret_cast<uint2*>(a.out + row1 * D + d) = make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
+      } else {
+        if (ok0) *reinterpret_cast<float4*>(a.part + (at + r0) * D + d) = x;
+        if (ok1) *reinterpret_cast<float4*>(a.part + (at + r1) * D + d) = y;
       }
-    if (!whole && c == 0) {
-      if (ok0) a.lse2[at + n] = l[0] == 0.f ? -INFINITY : m0 + log2f(l[0]);
-      if (ok1) a.lse2[at + n + 8] = l[2] == 0.f ? -INFINITY : m1 + log2f(l[2]);
+    };
+    if constexpr (kNarrow) {                                             // dims n D/8 + 4 i ..
+#pragma unroll
+      for (int i = 0; i < G::nt / 4; i++) {
+        const float (&u)[4] = o[2 * i], (&v)[4] = o[2 * i + 1];
+        put(n * (D / 8) + 4 * i, make_float4(u[0] * inv0, u[2] * inv0, v[0] * inv0, v[2] * inv0), make_float4(u[1] * inv1, u[3] * inv1, v[1] * inv1, v[3] * inv1));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int i = 0; i < G::nt / 4; i++)                              // dims (2 c + e) D/8 + 4 i ..
+          put((2 * c + e) * (D / 8) + 4 * i, make_float4(o[4 * i][e] * inv0, o[4 * i + 1][e] * inv0, o[4 * i + 2][e] * inv0, o[4 * i + 3][e] * inv0),
+              make_float4(o[4 * i][2 + e] * inv1, o[4 * i + 1][2 + e] * inv1, o[4 * i + 2][2 + e] * inv1, o[4 * i + 3][2 + e] * inv1));
+    }
+    if (!whole && (kNarrow ? n == 0 : c == 0)) {
+      if (ok0) a.lse2[at + r0] = sum0 == 0.f ? -INFINITY : m0 + log2f(sum0);
+      if (ok1) a.lse2[at + r1] = sum1 == 0.f ? -INFINITY : m1 + log2f(sum1);
     }
     if (left == 0) break;
   }
@@ -525,7 +582,7 @@ __global__ void __launch_bounds__(i4_join_threads(kSplit)) gqa_int4_join_kernel(
   if (r >= rows) return;                                                 // (kSplit: the whole CTA)
   constexpr int kBatch = 8, step = kSplit ? GR : 1;                      // loads in flight; pieces between a group's
   const int i0 = kSplit ? grp : 0;
-  auto place = [&](int i) { return ((long long)(first + i) * 2 + (i == 0)) * 16 + r; };
+  auto place = [&](int i) { return ((long long)(first + i) * 2 + (i == 0)) * a.rows + r; };
   float m = -INFINITY, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int b = i0; b < pieces; b += kBatch * step) {
@@ -577,44 +634,53 @@ __global__ void __launch_bounds__(i4_join_threads(kSplit)) gqa_int4_join_kernel(
 using namespace ne;
 
 namespace {
-template <int D, bool kPlain> cudaError_t launch_i4_main(const I4Args& a, cudaStream_t st) {
+template <int D, int R, bool kPlain> cudaError_t launch_i4_main(const I4Args& a, cudaStream_t st) {
   static bool configured[64] = {};                                       // per device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !configured[dev]) {
-    e = cudaFuncSetAttribute(gqa_int4_kernel<D, kPlain>, cudaFuncAttributeMaxDynamicSharedMemorySize, I4Geo<D>::smem);
+    e = cudaFuncSetAttribute(gqa_int4_kernel<D, R, kPlain>, cudaFuncAttributeMaxDynamicSharedMemorySize, I4Geo<D, R>::smem);
     if (e != cudaSuccess) return e;
     if (dev < 64) configured[dev] = true;
   }
-  return launch_pdl(gqa_int4_kernel<D, kPlain>, dim3((unsigned)(a.shares / kI4Warps)), dim3(kI4Threads), I4Geo<D>::smem, st, a);
+  return launch_pdl(gqa_int4_kernel<D, R, kPlain>, dim3((unsigned)(a.shares / kI4Warps)), dim3(kI4Threads), I4Geo<D, R>::smem, st, a);
+}
+template <int D, int R> cudaError_t launch_i4_rows(const I4Args& a, cudaStream_t st) {
+  return a.block_size % I4Geo<D, R>::keys == 0 ? launch_i4_main<D, R, true>(a, st) : launch_i4_main<D, R, false>(a, st);
 }
 template <int D> int launch_i4(const I4Args& a, int tiles, cudaStream_t st) {
-  const cudaError_t e = a.block_size % I4Geo<D>::keys == 0 ? launch_i4_main<D, true>(a, st) : launch_i4_main<D, false>(a, st);
+  const cudaError_t e = a.rows == 8 ? launch_i4_rows<D, 8>(a, st) : launch_i4_rows<D, 16>(a, st);
   if (e != cudaSuccess) return (int)e;
-  // pieces of a row tile: where they are many, a CTA per row shares them (us of both forms, 1184 shares: 8 row tiles 2.6 / 8.2, 120 row tiles 7.8 / 2.9)
-  if (a.shares > 16 * tiles) return (int)launch_pdl(gqa_int4_join_kernel<D, true>, dim3((unsigned)tiles, 16), dim3(i4_join_threads(true)), 0, st, a);
-  return (int)launch_pdl(gqa_int4_join_kernel<D, false>, dim3((unsigned)tiles, D / 32), dim3(i4_join_threads(false)), 0, st, a);
+  // Many pieces a row tile: a CTA per row shares them.  us of attention with a group per row / a CTA per row, 1184 shares, 64 / 4 heads of 128: 4 row tiles 99 / 38,
+  // 8: 84 / 53, 32: 59 / 60, 64: 39 / 51, 512: 89 / 193.
+  if (a.shares > 32 * tiles) return (int)launch_pdl(gqa_int4_join_kernel<D, true>, dim3((unsigned)tiles, a.rows), dim3(i4_join_threads(true)), 0, st, a);
+  const int rows_a_cta = i4_join_threads(false) / (D / 4);
+  return (int)launch_pdl(gqa_int4_join_kernel<D, false>, dim3((unsigned)tiles, (a.rows + rows_a_cta - 1) / rows_a_cta), dim3(i4_join_threads(false)), 0, st, a);
 }
 }  // namespace
 
-// Shares of the work that an SM's CTAs hold for heads of D (0: not built for them)
-extern "C" int ne_gqa_int4_shares(int D) { return kI4Warps * (D == 64 ? I4Geo<64>::ctas : D == 128 ? I4Geo<128>::ctas : D == 256 ? I4Geo<256>::ctas : 0); }
+// Shares of the work that an SM's CTAs hold for heads of D and row tiles of `rows` (0: not built for them)
+extern "C" int ne_gqa_int4_shares(int D, int rows) {
+  if (rows != 8 && rows != 16) return 0;
+  return kI4Warps * (D == 64 ? I4Geo<64, 8>::ctas : D == 128 ? (rows == 8 ? I4Geo<128, 8>::ctas : I4Geo<128, 16>::ctas) : D == 256 ? I4Geo<256, 8>::ctas : 0);
+}
 
-// q bf16 [T, Hq, D] with rows q_ld elements apart (8-byte aligned); k / v uint8 [num_blocks, Hkv, block_size (D/2 + D/32)].  shares: of the work, a multiple of 4, each with
-// two places of 16 rows in part fp32 [shares, 2, 16, D] and lse2 fp32 [shares, 2, 16].  tiles: an upper bound of the row tiles, the sum over sequences of
-// ceil(q_len / tq) Hkv ceil(g / 16), tq = max(1, 16 / g); cuts int32 [1 + tiles, 4].
+// q bf16 [T, Hq, D] with rows q_ld elements apart (8-byte aligned); k / v uint8 [num_blocks, Hkv, block_size (D/2 + D/32)].  rows: of a row tile, 8 or 16.  shares: of the work, a multiple of 4, each with
+// two places of them in part fp32 [shares, 2, rows, D] and lse2 fp32 [shares, 2, rows].  tiles: an upper bound of the row tiles, the sum over sequences of
+// ceil(q_len / tq) Hkv ceil(g / rows), tq = max(1, rows / g); cuts int32 [1 + tiles, 4].
 extern "C" int ne_gqa_int4(const void* q, long long q_ld, const void* k, const void* v, int num_blocks, int block_size, const int* block_tables, long long bt_ld, int bt_width,
-                           const int* cu_seqlens_q, const int* context_lens, int num_seqs, int T, int Hq, int Hkv, int D, int shares, int tiles, int window, float scale,
+                           const int* cu_seqlens_q, const int* context_lens, int num_seqs, int T, int Hq, int Hkv, int D, int rows, int shares, int tiles, int window, float scale,
                            void* out, float* part, float* lse2, void* cuts, cudaStream_t st) {
   if (T <= 0 || num_seqs <= 0) return 0;
   if (Hkv < 1 || Hq < Hkv || Hq % Hkv || num_blocks < 1 || bt_width < 1 || shares < kI4Warps || shares % kI4Warps || shares >= 32768 || tiles < 1 || !part || !lse2 || !cuts)
     return 1001;
+  if (rows != 8 && rows != 16) return 1003;
   if (!(block_size == 16 || block_size == 32 || (block_size > 0 && block_size % 64 == 0))) return 1002;
   I4Args a{};
   a.q = (const __nv_bfloat16*)q; a.q_ld = q_ld; a.k = (const uint8_t*)k; a.v = (const uint8_t*)v; a.num_blocks = num_blocks; a.block_size = block_size;
   a.block_tables = block_tables; a.bt_ld = bt_ld; a.bt_width = bt_width; a.cu_seqlens_q = cu_seqlens_q; a.context_lens = context_lens; a.num_seqs = num_seqs;
-  a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.g = Hq / Hkv; a.tq = a.g >= 16 ? 1 : 16 / a.g; a.head_tiles = (a.g + 15) / 16; a.shares = shares; a.max_tiles = tiles;
+  a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.g = Hq / Hkv; a.rows = rows; a.tq = a.g >= rows ? 1 : rows / a.g; a.head_tiles = (a.g + rows - 1) / rows; a.shares = shares; a.max_tiles = tiles;
   a.window = window > 0 ? window : 0; a.scale_log2 = scale * 1.4426950408889634f;
   a.out = (__nv_bfloat16*)out; a.part = part; a.lse2 = lse2; a.cuts = (int4*)cuts;
   switch (D) {

@@ -5,7 +5,7 @@
 //
 // Bound by latency: a decode step reads and writes tens of KB.  One launch: every CTA takes the prefix sum of all rows itself (a few hundred values
 // that sit in L2) instead of a scan kernel in front, then the CTAs share tokens and table entries; a token finds its sequence by a binary search in
-// shared memory.
+// shared memory.  Measured (B200, in a graph): 128 decode rows of 64 pages 3.3 us, 13 portions of 1260 tokens 2.9, one row of 2048 pages 2.9.
 #include "ptx.cuh"
 
 namespace ne {

@@ -874,9 +874,12 @@ def step_tables(q_lens, seq_lens, block_ids, block_offsets, block_size, num_toke
             and block_ids.is_contiguous() and block_offsets.is_contiguous()):
         q_lens, seq_lens, block_ids, block_offsets = (t.to(i32).contiguous() for t in (q_lens, seq_lens, block_ids, block_offsets))
     if out is None:
-        dev, i64, empty = q_lens.device, torch.int64, torch.empty
-        cu, ctx, last = empty(rows + 1, dtype=i32, device=dev), empty(rows, dtype=i32, device=dev), empty(rows, dtype=i32, device=dev)
-        pos, slot, table = empty(num_tokens, dtype=i64, device=dev), empty(num_tokens, dtype=i64, device=dev), empty(rows, max_blocks, dtype=i32, device=dev)
+        # one allocation: what has 64 bits, then the block tables and the vectors
+        words = 4 * num_tokens + rows * (max_blocks + 3) + 1
+        buf = torch.empty(words, dtype=i32, device=q_lens.device)
+        wide, table, cu, ctx, last = buf.split_with_sizes([4 * num_tokens, rows * max_blocks, rows + 1, rows, rows])
+        pos, slot = wide.view(torch.int64).split_with_sizes([num_tokens, num_tokens])
+        table = table.view(rows, max_blocks)
         ld = max_blocks
     else:
         sizes = [(rows + 1,), (rows,), (num_tokens,), (num_tokens,), (rows, max_blocks), (rows,)]

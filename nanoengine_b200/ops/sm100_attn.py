@@ -284,6 +284,7 @@ def gqa_attention_paged(q, k_cache, v_cache, block_tables, cu_seqlens_q, context
 
 INT4_CALLS = [0]             # calls of the kernel that reads 4-bit pages itself
 _INT4_SHARES = {}
+_INT4_EXPANDED_BYTES = 2 << 30       # what a step over 4-bit pages may take for pages in bf16
 
 
 def _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale, window: int):
@@ -307,23 +308,31 @@ def _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, sca
         return torch.zeros(T, Hq, D, dtype=torch.bfloat16, device=dev)
     if q.dtype != torch.bfloat16 or q.stride(2) != 1 or q.stride(1) != D or q.stride(0) % 4 or q.data_ptr() % 8:
         q = q.to(torch.bfloat16).clone(memory_format=torch.contiguous_format)
-    if T * g >= 128 * B and (g % 4 == 0 or g == 1 and Hq % 4 == 0) and g <= 128:
+    # Many rows a sequence: unpacking for every 16 of them costs more than expanding the context once.  us of the kernel / of expanding, then the prompt kernel: 32 x 4096 keys,
+    # 64 / 4 heads of 128: 64 rows 92 / 157, 128: 166 / 163, 256: 307 / 174; 16 / 2 heads of 256: 64: 111 / 185, 128: 194 / 182; 16 x 4096, 16 / 2 heads of 64: 256: 57 / 83,
+    # 512: 100 / 103; 4 x 4096, 64 / 4 of 128: 128: 38 / 57, 512: 89 / 75.  The expanded pages take 15 times the room of the 4-bit ones: not where that is more than 2 GB.
+    if (T * g >= (512 if D == 64 else 128) * B and (g % 4 == 0 or g == 1 and Hq % 4 == 0) and g <= 128
+            and 4 * B * W * bs * Hkv * D <= _INT4_EXPANDED_BYTES):
         k, v, bt, cl = _k.kv4_expand(k_cache, v_cache, bt, cl, D)
         return gqa_attention_paged(q, k, v, bt, cu, cl, scale, window)
+    # Row tiles of 8 where a sequence has no more rows of a kv head, else of 16.  us of 16 / 8: 128 x 4096 keys, 32 / 8 heads of 128: 159 / 117, of 64: 96 / 78;
+    # 60 x 3000, 16 / 2 heads of 256: 53 / 43.
+    rows = 8 if T * g <= 8 * B else 16
     # equal shares of the batch's work, one for every warp that is resident at once, but no more than its tiles of keys need
-    per_sm = _INT4_SHARES.get(D)
+    per_sm = _INT4_SHARES.get((D, rows))
     if per_sm is None:
-        per_sm = _INT4_SHARES[D] = _k.lib().ne_gqa_int4_shares(D)
-    tq = 16 // g if g < 16 else 1
-    tiles = min(T, T // tq + B) * Hkv * -(-g // 16)
+        per_sm = _INT4_SHARES[D, rows] = _k.lib().ne_gqa_int4_shares(D, rows)
+    tq = rows // g if g < rows else 1
+    tiles = min(T, T // tq + B) * Hkv * -(-g // rows)
     shares = min(_sms() * per_sm, -(-tiles * -(-W * bs // (32 if D == 256 else 64)) // 8) * 4)
     out = torch.empty(T, Hq, D, dtype=torch.bfloat16, device=dev)
     # partial results, their statistics and the row tiles that cuts run through
-    part = torch.empty(shares * 32 * (D + 1) + 4 * (tiles + 1), dtype=torch.float32, device=dev)
+    part = torch.empty(shares * 2 * rows * (D + 1) + 4 * (tiles + 1), dtype=torch.float32, device=dev)
     at = part.data_ptr()
-    _k._ck(_k._fn("ne_gqa_int4", "plppiipli" + "ppi" + "iiiiiii" + "f" + "ppppp")(
+    _k._ck(_k._fn("ne_gqa_int4", "plppiipli" + "ppi" + "iiiiiiii" + "f" + "ppppp")(
         q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], bs, bt.data_ptr(), bt.stride(0), W, cu.data_ptr(), cl.data_ptr(), B,
-        T, Hq, Hkv, D, shares, tiles, window if window > 0 else 0, scale, out.data_ptr(), at, at + shares * 128 * D, at + shares * 128 * (D + 1), _k._stream()), "ne_gqa_int4")
+        T, Hq, Hkv, D, rows, shares, tiles, window if window > 0 else 0, scale, out.data_ptr(), at, at + shares * 8 * rows * D, at + shares * 8 * rows * (D + 1), _k._stream()),
+        "ne_gqa_int4")
     INT4_CALLS[0] += 1
     _k.LAUNCHES[0] += 1
     return out
