@@ -261,6 +261,69 @@ def test_prompts(hq, hkv, dim, bs, new, ctx, window):
     assert bool((off <= 0).all()), float(off.max())
 
 
+# at most eight rows of a kv head per sequence: the products with keys and dims as their rows
+FEW_ROWS = [
+    # hq, hkv, dim, block size, new tokens, contexts, window
+    (8, 8, 128, 64, [1, 1, 1], [1, 64, 193], 0),
+    (4, 2, 128, 16, [1, 1], [17, 300], 0),
+    (6, 2, 64, 32, [1, 1], [95, 96], 0),
+    (10, 2, 256, 64, [1], [1025], 0),
+    (6, 1, 128, 192, [1, 1], [700, 191], 0),
+    (14, 2, 64, 64, [1, 1], [2000, 3], 0),
+    (8, 1, 256, 16, [1, 1], [33, 31], 0),
+    (32, 4, 128, 64, [1, 1], [900, 64], 100),
+    (8, 2, 64, 16, [1], [77], 1),
+    (16, 8, 256, 128, [4], [260], 130),
+    (4, 2, 128, 64, [4, 1, 0, 3], [4, 130, 9, 2], 0),                  # more new tokens than context: the first see nothing
+    (4, 1, 128, 64, [1, 0, 1], [0, 0, 5000], 0),
+    (12, 1, 64, 64, [1, 0], [400, 5], 0),                              # fewer tokens than sequences: two tiles of the group's heads
+    (32, 8, 128, 64, [1], [40000], 0),
+    (16, 2, 256, 64, [1] * 9, [3000 + 7 * i for i in range(9)], 0),
+]
+
+
+@pytest.mark.parametrize("hq,hkv,dim,bs,new,ctx,window", FEW_ROWS)
+def test_few_rows(hq, hkv, dim, bs, new, ctx, window):
+    assert sum(new) * (hq // hkv) <= 8 * len(new)
+    args, (out, spread, mass, top) = run_attention(hq, hkv, dim, bs, new, ctx, window, seed=2)
+    got = ops.gqa_attention_paged(*args)
+    off = (got.double() - out).abs() - attention_bound(out, spread, mass, top)
+    assert bool((off <= 0).all()), float(off.max())
+
+
+@pytest.mark.parametrize("hq,hkv,dim,bs,new,ctx,window", [(64, 4, 128, 64, [70, 33], [70, 200], 0), (16, 4, 64, 16, [300], [411], 0)])
+def test_prompts_with_and_without_room_for_bf16_pages(hq, hkv, dim, bs, new, ctx, window, monkeypatch):
+    from nanoengine_b200.ops import sm100_attn
+    args, (out, spread, mass, top) = run_attention(hq, hkv, dim, bs, new, ctx, window, seed=3)
+    bound = attention_bound(out, spread, mass, top)
+    for room in (sm100_attn._INT4_EXPANDED_BYTES, 0):
+        monkeypatch.setattr(sm100_attn, "_INT4_EXPANDED_BYTES", room)
+        before = sm100_attn.INT4_CALLS[0]
+        got = ops.gqa_attention_paged(*args)
+        assert (sm100_attn.INT4_CALLS[0] == before) == (room > 0)
+        assert bool(((got.double() - out).abs() <= bound).all())
+
+
+def test_a_query_that_is_no_number_among_few_rows_stays_its_own():
+    args, (out, spread, mass, top) = run_attention(16, 4, 128, 64, [1, 1], [90, 300], 0, seed=6)
+    q = args[0].clone()
+    q[0, 3], q[1, 5] = float("nan"), float("inf")
+    got = ops.gqa_attention_paged(q, *args[1:])
+    hurt = torch.zeros(got.shape[:2], dtype=torch.bool, device=DEV)
+    hurt[0, 3] = hurt[1, 5] = True
+    assert bool(got[hurt].isnan().all())
+    assert bool(((got.double() - out).abs() <= attention_bound(out, spread, mass, top))[~hurt].all())
+
+
+def test_boundaries_past_the_last_query_row_write_nothing_behind_it():
+    """Query boundaries that name more rows than there are: the rows there are get their results, the kernel stays inside its tables."""
+    args, (out, spread, mass, top) = run_attention(8, 2, 128, 64, [1, 2], [90, 300], 0, seed=7)
+    q, kc, vc, table, _, ctx, scale, _ = args
+    got = ops.gqa_attention_paged(q, kc, vc, table, torch.tensor([0, 1, 40], dtype=torch.int32, device=DEV), ctx, scale)
+    assert bool(((got[:1].double() - out[:1]).abs() <= attention_bound(out, spread, mass, top)[:1]).all())
+    assert got.shape == q.shape
+
+
 @pytest.mark.parametrize("new", [[1, 1], [80, 90]])
 def test_pages_outside_the_cache_read_as_zeros_and_contexts_end_with_their_tables(new):
     g = gen(8)
