@@ -535,6 +535,20 @@ def case_gqa(B, ctx, q_len, Hq, Hkv, D=128, bs=64):
     return fn, B * ctx * Hkv * D * 4 + T * Hq * D * 4, 4.0 * T * Hq * causal * D
 
 
+def case_gqa_int4(B, ctx, q_len, Hq, Hkv, D=128):
+    """`case_gqa` over a 4-bit cache: codes and scale bytes in place of bf16 rows."""
+    T, pages = B * q_len, (ctx + 63) // 64
+    row = sm100.kv4_page_bytes(D, 64)
+    k = torch.randint(0, 256, (B * pages, Hkv, row), dtype=torch.uint8, device="cuda")
+    v = torch.randint(0, 256, (B * pages, Hkv, row), dtype=torch.uint8, device="cuda")
+    k[..., 64 * D // 2:], v[..., 64 * D // 2:] = 96, 96
+    bt = torch.randperm(B * pages, device="cuda").to(torch.int32).view(B, pages)
+    q = torch.randn(T, Hq, D, device="cuda", dtype=torch.bfloat16)
+    cu = torch.arange(B + 1, dtype=torch.int32, device="cuda") * q_len
+    cl = torch.full((B,), ctx, dtype=torch.int32, device="cuda")
+    nbytes = 2 * B * ctx * Hkv * (D // 2 + D // 32)
+    return (lambda: sm100_attn.gqa_attention_paged(q, k, v, bt, cu, cl, D ** -0.5)), nbytes, 4.0 * T * Hq * D * (ctx - q_len / 2)
+
 def case_moe_layer(T, E, topk=8, H=7168, I=2048):
     x = torch.randn(T, H, device="cuda", dtype=torch.bfloat16)
     w13, w2 = rand_fp8(E, 2 * I, H), rand_fp8(E, H, I)
@@ -598,6 +612,8 @@ def build_cases(args):
         "indexer_prefill_4k": lambda: case_indexer(1, 8192, q_len=4096),
         "gqa_decode_tp8": lambda: case_gqa(256, 4352, 1, 8, 1),          # Qwen3-235B per rank at TP8: 8 q heads, 1 kv head
         "gqa_decode_tp1": lambda: case_gqa(64, 4352, 1, 64, 4),
+        "gqa_int4_decode_tp8": lambda: case_gqa_int4(256, 4352, 1, 8, 1),
+        "gqa_int4_decode_tp1": lambda: case_gqa_int4(64, 4352, 1, 64, 4),
         "gqa_prefill_tp8": lambda: case_gqa(4, 4096, 4096, 8, 1),
         "absorb_k_decode": lambda: case_absorb(128, "k"),
         "absorb_v_decode": lambda: case_absorb(128, "v"),

@@ -30,7 +30,7 @@
 namespace ne {
 
 constexpr int kKernelI4 = 31;
-constexpr int kI4Warps = 4, kI4Threads = 32 * kI4Warps;
+constexpr int kI4Warps = 4, kI4Threads = 32 * kI4Warps, kI4Slots = 2;
 
 struct I4Args {
   const __nv_bfloat16* q; long long q_ld;              // [T, Hq, D], rows q_ld apart
@@ -47,7 +47,7 @@ struct I4Args {
 
 template <int D, int R> struct I4Geo {                                  // R: rows of a row tile, 8 or 16
   static constexpr int keys = D == 256 ? 32 : 64;                       // of a tile
-  static constexpr int slots = D == 256 || (D == 128 && R == 8) ? 2 : 3;   // of a warp's ring
+  static constexpr int slots = kI4Slots;                                // of a warp's ring (three: 43 us where two take 40 for 33 x 2504 keys, four tokens)
   static constexpr int ctas = D == 64 || (D == 128 && R == 8) ? 3 : 2;  // resident per SM
   static constexpr int row = D / 2, srow = D / 32;                      // bytes of a row's codes and scales
   static constexpr int codes = keys * row, half = codes + keys * srow, stage = 2 * half;
@@ -81,10 +81,9 @@ template <int KEYS> __device__ __forceinline__ I4Seq i4_load(const I4Args& a, in
 // Units of a share: equal ones, but no less than two
 __device__ __forceinline__ int i4_share(long long total, int shares) { return (int)max((total + shares - 1) / shares, 2ll); }
 
-constexpr int kI4MaxSlots = 3;
 struct I4Shared {
-  uint64_t bar[kI4Warps * kI4MaxSlots];                                  // a slot's tile has landed
-  uint32_t bad[kI4Warps * kI4MaxSlots];                                  // pieces of it whose page lies outside the cache
+  uint64_t bar[kI4Warps * kI4Slots];                                  // a slot's tile has landed
+  uint32_t bad[kI4Warps * kI4Slots];                                  // pieces of it whose page lies outside the cache
   int abort, tiles[kI4Warps];
   long long units[kI4Warps];
   int4 start[kI4Warps];                                                  // where a warp's share starts: sequence, (row tile, head) of it, unit of that; row tiles in front of the sequence

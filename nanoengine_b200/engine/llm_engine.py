@@ -143,7 +143,12 @@ class LLMEngine:
             self._with_axes.add(seq_id)
         self._next_seq_id = max(self._next_seq_id, seq_id) + 1
         sp = sampling_params or C.SamplingParams()
-        return self.scheduler.add_request(C.RequestIn(seq_id, list(prompt_token_ids), sp, 0, [slot] if slot >= 0 else None))
+        try:
+            return self.scheduler.add_request(C.RequestIn(seq_id, list(prompt_token_ids), sp, 0, [slot] if slot >= 0 else None))
+        except Exception:
+            if axes:
+                self._release_axes(seq_id)
+            raise
 
     # ---- file-backed KV tier ------------------------------------------------------------------
     def _l3_import(self, prompt_token_ids: List[int]) -> int:

@@ -434,7 +434,8 @@ def gqa_kv_gather(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Ten
 
 
 def gqa_kv_store(k_cache, v_cache, slot_mapping, k, v) -> None:
-    """k_cache/v_cache [blocks, block_size, kv_heads, head_dim], or 4-bit pages uint8 [blocks, kv_heads, kv4_page_bytes] (there slot -1 writes nothing)."""
+    """k_cache/v_cache [blocks, block_size, kv_heads, head_dim], or 4-bit pages uint8 [blocks, kv_heads, kv4_page_bytes] (there slot -1 writes nothing).
+    Slots are distinct: a slot named twice holds parts of either row."""
     if k_cache.dtype == torch.uint8:
         _kv4_store(k_cache, slot_mapping, k)
         _kv4_store(v_cache, slot_mapping, v)
@@ -724,7 +725,7 @@ def gqa_attention_paged(q, k_cache, v_cache, block_tables, cu_seqlens_q, context
     """q [T, Hq, D]; caches [blocks, block_size, Hkv, D]; causal; returns [T, Hq, D].  `window` > 0: a query at position p sees
     key positions (p - window, p] only (sliding-window layers, reference layers/backends/attention/base.py:527-707).
     uint8 caches hold 4-bit rows, [blocks, Hkv, kv4_page_bytes]: there a page id outside the cache reads as rows of zeros, a context is cut off where its
-    block table ends, and a query that sees no key gives zeros."""
+    block table ends, and a query that sees no key gives zeros; rows of q behind the last sequence's are unspecified."""
     T, Hq, D = q.shape
     if k_cache.dtype == torch.uint8:
         return _gqa_attention_kv4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale, window)
@@ -761,6 +762,8 @@ def check_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor) -> 
 def _gqa_attention_kv4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale, window: int) -> torch.Tensor:
     T, Hq, D = q.shape
     Hkv, bs = check_kv4(q, k_cache, v_cache)
+    if not scale > 0:
+        raise ValueError("the scale of the scores is positive")
     out = torch.zeros(T, Hq, D, dtype=torch.float32, device=q.device)
     for i in range(cu_seqlens_q.numel() - 1):
         lo, hi = max(0, int(cu_seqlens_q[i])), min(T, int(cu_seqlens_q[i + 1]))
