@@ -87,6 +87,7 @@ struct I4Shared {
   int abort, tiles[kI4Warps];
   long long units[kI4Warps];
   int4 start[kI4Warps];                                                  // where a warp's share starts: sequence, (row tile, head) of it, unit of that; row tiles in front of the sequence
+  int3 seq[kI4Warps];                                                    // begin, end and context of that sequence
   int beg[kI4Threads], end[kI4Threads], ctx[kI4Threads];                 // what the sequences from the first of these on are
 };
 
@@ -129,12 +130,14 @@ template <int KEYS> __device__ __forceinline__ I4Total i4_plan(const I4Args& a, 
     long long base = before;
     int t = before_t;
     for (int i = s0;; i++) {
-      const I4Seq s = i4_load<KEYS>(a, i);
+      const int3 x = make_int3(a.cu_seqlens_q[i], a.cu_seqlens_q[i + 1], a.context_lens[i]);
+      const I4Seq s = i4_seq<KEYS>(a, x.x, x.y, x.z);
       const int n = s.tiles * heads;
       const long long end = base + (long long)n * s.per_tile;
       if (u < end || i + 1 >= s1) {
         const int th = (int)((u - base) / s.per_tile);
         sh.start[w] = make_int4(i, th, (int)(u - base - (long long)th * s.per_tile), t);
+        sh.seq[w] = x;
         break;
       }
       base = end;
@@ -163,10 +166,10 @@ template <int KEYS> __device__ __forceinline__ void i4_fill(const I4Args& a, I4P
   p.t_end = p.n_tok > 0 ? min(p.s.first + p.unit + p.units, max_limit >= 0 ? max_limit / KEYS + 1 : 0) : 0;
 }
 // the piece that a share starts with; `left` units the share has
-template <int KEYS> __device__ __forceinline__ I4Piece i4_first(const I4Args& a, const int4& at, int left) {
+template <int KEYS> __device__ __forceinline__ I4Piece i4_first(const I4Args& a, const int4& at, const int3& seq, int left) {
   I4Piece p;
   p.seq = at.x;
-  p.s = i4_load<KEYS>(a, p.seq);
+  p.s = i4_seq<KEYS>(a, seq.x, seq.y, seq.z);
   const int heads = a.Hkv * a.head_tiles, head = at.y % heads;
   p.unit = at.z;
   p.index = at.w + at.y;
@@ -240,9 +243,6 @@ __global__ void __launch_bounds__(kI4Threads, I4Geo<D, R>::ctas) gqa_int4_kernel
   if (blockIdx.x == 0 && threadIdx.x == 0) a.cuts[0] = make_int4(total.tiles, 0, 0, 0);
   const int share = total.share;
   if ((long long)blockIdx.x * kI4Warps * share >= total.units) return;
-  if (const int i = sh.start[0].x + threadIdx.x; i < a.num_seqs) {
-    sh.beg[threadIdx.x] = a.cu_seqlens_q[i]; sh.end[threadIdx.x] = a.cu_seqlens_q[i + 1]; sh.ctx[threadIdx.x] = a.context_lens[i];
-  }
   const int mine = blockIdx.x * kI4Warps + warp;                         // this warp's share
   const long long u0 = (long long)mine * share;
   int left = (int)min((long long)share, max(0ll, total.units - u0));         // units of it still to do
@@ -303,16 +303,23 @@ __global__ void __launch_bounds__(kI4Threads, I4Geo<D, R>::ctas) gqa_int4_kernel
   };
 
   I4Piece p;
-  if (left > 0) p = i4_first<G::keys>(a, sh.start[warp], left);
+  int slot = 0, phase = 0;                                               // of the next tile to read
+  if (left > 0) {
+    p = i4_first<G::keys>(a, sh.start[warp], sh.seq[warp], left);
+    if (p.t_begin < p.t_end) fetch(p, p.t_begin, 0, page_of(p, p.t_begin));
+  }
+  if (const int i = sh.start[0].x + threadIdx.x; i < a.num_seqs) {
+    sh.beg[threadIdx.x] = a.cu_seqlens_q[i]; sh.end[threadIdx.x] = a.cu_seqlens_q[i + 1]; sh.ctx[threadIdx.x] = a.context_lens[i];
+  }
   __syncthreads();                                                       // the table of sequences
   if (left == 0) return;
-  int slot = 0, phase = 0;                                               // of the next tile to read
-#pragma unroll 1
-  for (int i = 0; i < ST; i++) if (p.t_begin + i < p.t_end) fetch(p, p.t_begin + i, i, page_of(p, p.t_begin + i));
+  // The second tile is asked for when the first is there: all warps start at once, and the first tiles of some would come behind the second ones of others
+  bool lead = p.t_begin + 1 < p.t_end;
+  int id = page_of(p, p.t_begin + 1);
 
   while (true) {
     const int n_tok = p.n_tok, gh = p.gh, head0 = p.head0, tok0 = p.tok0, base_limit = p.base_limit, max_limit = p.base_limit + p.n_tok - 1;
-    int id = page_of(p, p.t_begin + ST);
+    if (!lead) id = page_of(p, p.t_begin + ST);
 
     // this lane's two query rows (fragment rows n and n + 8): token and head
     // (narrow: it loads row n and has results of rows 2 c and 2 c + 1)
@@ -364,6 +371,11 @@ __global__ void __launch_bounds__(kI4Threads, I4Geo<D, R>::ctas) gqa_int4_kernel
       if (!__all_sync(0xffffffffu, landed)) {                            // a copy has not come: let the others land before the block's memory goes
         for (int i = 0; i < 2000; i++) __nanosleep(1000);
         return;
+      }
+      if (lead) {
+        fetch(p, tile + 1, 1, id);
+        id = page_of(p, tile + ST);
+        lead = false;
       }
       if (const uint32_t bad = sh.bad[warp * ST + slot]) {               // pages outside the cache read as zeros: code 8
         const int piece = min(a.block_size, G::keys);
