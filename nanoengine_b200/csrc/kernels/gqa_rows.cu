@@ -404,12 +404,16 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(const uint8_t* __restri
 
 // The contexts of all sequences as bf16 pages of 64 tokens of their own, [B * width, 64, Hkv, D], page p of sequence i at i * width + p, with that table and
 // the context lengths (cut off where their block tables end).  Pages outside the cache read as zeros, and so do keys behind a context that share a page
-// with it; pages behind a context are left out.
+// with it; pages behind a context are left out.  A CTA takes a page of a head: its threads find the rows' places once, then each unpacks words of 8 dims, so that
+// neighbouring lanes store neighbouring 16 bytes.
+template <int D>
 __global__ void __launch_bounds__(256) kv4_expand_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, int num_blocks,
                                                         const int* __restrict__ tables, long long bt_ld, int bt_width, const int* __restrict__ ctx,
                                                         __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int* __restrict__ out_tables,
-                                                        int* __restrict__ out_ctx, int width, int Hkv, int D, int block_size) {
+                                                        int* __restrict__ out_ctx, int width, int Hkv, int block_size) {
   pdl_wait(); pdl_trigger();
+  constexpr int words = D / 8, items = 64 * words / 256, kFlight = items < 4 ? items : 4;        // words of a thread, in flight
+  __shared__ long long s_code[64], s_scale[64];                          // where a row's codes and scales begin, -1: zeros
   const int seq = blockIdx.y, p = blockIdx.x, h = blockIdx.z;
   const long long at = (long long)seq * width + p;
   const int n = (int)min((long long)ctx[seq], (long long)bt_width * block_size);
@@ -418,29 +422,38 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(const uint8_t* __restri
     if (p == 0) out_ctx[seq] = n;
   }
   if (p * 64 >= n) return;
-  const int words = D / 8;
-  constexpr int kFlight = 4;                                             // words of a thread in flight
-  for (int i0 = threadIdx.x; i0 < 64 * words; i0 += 256 * kFlight) {
+  if (threadIdx.x < 64) {
+    const int key = p * 64 + threadIdx.x;
+    long long code = -1, scale = -1;
+    if (key < n) {
+      const int page = key / block_size, tok = key - page * block_size, id = tables[(long long)seq * bt_ld + page];
+      if (id >= 0 && id < num_blocks && NE_INDEX_OK(id, BK_CACHE_PAGES, 30, __LINE__)) {
+        const long long base = ((long long)id * Hkv + h) * ((long long)block_size * (D / 2 + D / 32));
+        code = base + tok * (D / 2);
+        scale = base + block_size * (D / 2) + tok * (D / 32);
+      }
+    }
+    s_code[threadIdx.x] = code;
+    s_scale[threadIdx.x] = scale;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i0 = 0; i0 < items; i0 += kFlight) {
     uint32_t kw[kFlight], vw[kFlight], ks[kFlight], vs[kFlight];
 #pragma unroll
     for (int u = 0; u < kFlight; u++) {
-      const int i = i0 + u * 256, r = i / words, j = i - r * words, key = p * 64 + r;
+      const int i = threadIdx.x + (i0 + u) * 256, r = i / words, j = i % words;
+      const long long code = s_code[r], scale = s_scale[r] + j / 4;
       kw[u] = vw[u] = 0x88888888u;                                       // zeros
       ks[u] = vs[u] = 0;
-      if (r < 64 && key < n) {
-        const int id = tables[(long long)seq * bt_ld + key / block_size], tok = key % block_size;
-        if (id >= 0 && id < num_blocks && NE_INDEX_OK(id, BK_CACHE_PAGES, 30, __LINE__)) {
-          const long long base = ((long long)id * Hkv + h) * ((long long)block_size * (D / 2 + D / 32));
-          const long long code = base + tok * (D / 2) + 4 * j, scale = base + block_size * (D / 2) + tok * (D / 32) + j / 4;
-          kw[u] = *reinterpret_cast<const uint32_t*>(k_cache + code); ks[u] = k_cache[scale];
-          vw[u] = *reinterpret_cast<const uint32_t*>(v_cache + code); vs[u] = v_cache[scale];
-        }
+      if (code >= 0) {
+        kw[u] = *reinterpret_cast<const uint32_t*>(k_cache + code + 4 * j); ks[u] = k_cache[scale];
+        vw[u] = *reinterpret_cast<const uint32_t*>(v_cache + code + 4 * j); vs[u] = v_cache[scale];
       }
     }
 #pragma unroll
     for (int u = 0; u < kFlight; u++) {
-      const int i = i0 + u * 256, r = i / words, j = i - r * words;
-      if (r >= 64) break;
+      const int i = threadIdx.x + (i0 + u) * 256, r = i / words, j = i % words;
       const long long dst = ((at * 64 + r) * Hkv + h) * D + 8 * j;
       *reinterpret_cast<uint4*>(k_out + dst) = kv4_word(kw[u], ks[u]);
       *reinterpret_cast<uint4*>(v_out + dst) = kv4_word(vw[u], vs[u]);
@@ -516,8 +529,11 @@ extern "C" int ne_kv4_gather(const void* k_cache, const void* v_cache, const lon
 extern "C" int ne_kv4_expand(const void* k_cache, const void* v_cache, int num_blocks, const int* tables, long long bt_ld, int bt_width, const int* ctx, int seqs, int width,
                              void* k_out, void* v_out, int* out_tables, int* out_ctx, int Hkv, int D, int block_size, cudaStream_t st) {
   if (seqs <= 0 || width <= 0) return 0;
-  if (num_blocks < 1 || Hkv < 1 || block_size < 1 || D < 32 || D % 32 || seqs > 65535 || Hkv > 65535 || (long long)width * 64 < (long long)bt_width * block_size ||
+  if (num_blocks < 1 || Hkv < 1 || block_size < 1 || seqs > 65535 || Hkv > 65535 || (long long)width * 64 < (long long)bt_width * block_size ||
       (long long)seqs * width >= (1ll << 31)) return 1001;
-  return (int)launch_pdl(kv4_expand_kernel, dim3((unsigned)width, (unsigned)seqs, (unsigned)Hkv), dim3(256), 0, st, (const uint8_t*)k_cache, (const uint8_t*)v_cache, num_blocks,
-                         tables, bt_ld, bt_width, ctx, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, out_tables, out_ctx, width, Hkv, D, block_size);
+  auto go = [&](auto kern) {
+    return (int)launch_pdl(kern, dim3((unsigned)width, (unsigned)seqs, (unsigned)Hkv), dim3(256), 0, st, (const uint8_t*)k_cache, (const uint8_t*)v_cache, num_blocks, tables,
+                           bt_ld, bt_width, ctx, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, out_tables, out_ctx, width, Hkv, block_size);
+  };
+  return D == 64 ? go(kv4_expand_kernel<64>) : D == 128 ? go(kv4_expand_kernel<128>) : D == 256 ? go(kv4_expand_kernel<256>) : 1002;
 }
