@@ -64,7 +64,8 @@ template <int L, typename R> __device__ __forceinline__ void norm_and_turn(R (&x
   for (int e = 0; e < 8; e++) ss += x[e] * x[e];
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const R r = norm ? rsqrt(ss / (R)(8 * L) + eps) : (R)1;
+  const R mean = ss / (R)(8 * L) + eps, r = norm ? rsqrt(mean) : (R)1;
+  const bool lost = norm && !(mean > (R)1e-30 && mean < (R)1e37);        // squares that 32 bits do not hold: no bound
   // Error in 32 bits, relative to the sum of the two magnitudes: 7 2^-24 of the mean (14 additions, halved by the root), 2^-22 of the root, 2^-24 each for
   // weight, factor, two products, sum and scaling: below 2^-20
 #pragma unroll
@@ -73,8 +74,8 @@ template <int L, typename R> __device__ __forceinline__ void norm_and_turn(R (&x
     x[e] = r * (a * t.ca[e] - b * t.sb[e]);
     x[4 + e] = r * (b * t.cb[e] + a * t.sa[e]);
     if (off) {
-      off[e] = (float)(r * (fabs(a * t.ca[e]) + fabs(b * t.sb[e]))) * 0x1p-20f;
-      off[4 + e] = (float)(r * (fabs(b * t.cb[e]) + fabs(a * t.sa[e]))) * 0x1p-20f;
+      off[e] = lost ? INFINITY : (float)(r * (fabs(a * t.ca[e]) + fabs(b * t.sb[e]))) * 0x1p-20f;
+      off[4 + e] = lost ? INFINITY : (float)(r * (fabs(b * t.cb[e]) + fabs(a * t.sa[e]))) * 0x1p-20f;
     }
   }
 }

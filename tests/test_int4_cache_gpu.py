@@ -147,6 +147,22 @@ def test_rows(T, hq, hkv, d, bs, sections, interleaved, norm, offset, int4):
 
 
 @pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("eps", [1e-6, 0.0])
+def test_key_rows_whose_squares_32_bits_do_not_hold(d, eps):
+    """Keys of 2^-70 to 2^100 (a row of ordinary size among them): the codes are those of the row in 64 bits all the same."""
+    T, hq, hkv, bs = 9, 2, 3, 16
+    g, qkv, qw, kw, pos, table = rows_inputs(T, hq, hkv, d, 1, d)
+    size = torch.tensor([-70, -64, -40, -1, 0, 30, 63, 64, 100], device=DEV)
+    qkv = (qkv.float() * torch.exp2(size.float())[:, None]).to(torch.bfloat16)
+    kc, vc = (torch.zeros(2, hkv, ops.kv4_page_bytes(d, bs), dtype=torch.uint8, device=DEV) for _ in range(2))
+    ops.gqa_qkv_prepare(qkv, hq, hkv, d, qw, kw, eps, False, pos[0], table, kc, vc, torch.arange(T, device=DEV))
+    x = qkv.view(T, -1, d)
+    for cache, want in ((kc, rows_exact(x[:, hq: hq + hkv], kw, eps, 0.0, pos, table, [d // 2], False)), (vc, x[:, hq + hkv:].double())):
+        most = 7 * 1.875 * 2.0 ** 15
+        assert torch.equal(cache_values(cache, d).flatten(0, 1)[:T], nearest(want.clamp(-most, most)))
+
+
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
 def test_store_alone_takes_strided_rows_and_extremes(d):
     g = gen(d)
     T, hkv, bs = 21, 3, 16
