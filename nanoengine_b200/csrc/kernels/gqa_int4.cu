@@ -21,8 +21,8 @@
 //
 // Bound by the chain unpack, product, softmax of two (three) warps a scheduler, not by HBM: cycles of a warp for a tile of 64 keys and 16 rows: waiting for copies 290,
 // scores 1460, maximum 290, values 1770, next copy 580; a product and the two pairs that feed it take 9.7 cycles of their pipes, of which none is full (matrix
-// 32 %, integer 31 %, issue slots 41 %).  Measured (B200, calls in a graph, us, GB/s of 6530): 128 x 4096 keys, 64 / 4 heads of 128 (16 rows): 88, 3240;
-// 32 / 8 heads (4 rows): 116, 4920; 2 x 131072 keys, 64 / 4: 52; 60 x 3000, 16 / 2 heads of 256: 42; 33 x 2504, four tokens, 32 / 8: 39; 1 x 1001: 10.  Slower: queries in shared memory, tiles of 32 keys, copies by cp.async, three CTAs per SM with 16 rows (they spill).  tcgen05 with the keys
+// 32 %, integer 31 %, issue slots 41 %).  Measured (B200, calls in a graph, us, GB/s of 6530): 128 x 4096 keys, 64 / 4 heads of 128 (16 rows): 86, 3320;
+// 32 / 8 heads (4 rows): 115, 4960; 2 x 131072 keys, 64 / 4: 50; 60 x 3000, 16 / 2 heads of 256: 40; 33 x 2504, four tokens, 32 / 8: 37; 1 x 1001: 10.  Slower: queries in shared memory, tiles of 32 keys, copies by cp.async, three CTAs per SM with 16 rows (they spill).  tcgen05 with the keys
 // unpacked into tensor memory and the values into shared memory, three CTAs per SM, a warp of its own for copies and products: 116 where this one takes 89; the
 // unpacked values cross shared memory twice, and barriers between unpacking, products and softmax leave the pipes idle.
 #include "kv4.cuh"
@@ -663,9 +663,9 @@ template <int D, int R> cudaError_t launch_i4_rows(const I4Args& a, cudaStream_t
 template <int D> int launch_i4(const I4Args& a, int tiles, cudaStream_t st) {
   const cudaError_t e = a.rows == 8 ? launch_i4_rows<D, 8>(a, st) : launch_i4_rows<D, 16>(a, st);
   if (e != cudaSuccess) return (int)e;
-  // Many pieces a row tile: a CTA per row shares them.  us of attention with a group per row / a CTA per row, 1184 shares, 64 / 4 heads of 128: 4 row tiles 95 / 35,
-  // 8: 82 / 52, 32: 58 / 58, 64: 36 / 49, 512: 88 / 192.
-  if (a.shares > 32 * tiles) return (int)launch_pdl(gqa_int4_join_kernel<D, true>, dim3((unsigned)tiles, a.rows), dim3(i4_join_threads(true)), 0, st, a);
+  // Many pieces a row tile: a CTA per row shares them.  us of attention with a group per row / a CTA per row, 1184 shares, 64 / 4 heads of 128: 4 row tiles 57 / 34,
+  // 8: 62 / 50, 32: 51 / 57, 64: 33 / 48, 512: 86 / 194.
+  if (a.shares > 64 * tiles) return (int)launch_pdl(gqa_int4_join_kernel<D, true>, dim3((unsigned)tiles, a.rows), dim3(i4_join_threads(true)), 0, st, a);
   const int rows_a_cta = i4_join_threads(false) / (D / 4);
   return (int)launch_pdl(gqa_int4_join_kernel<D, false>, dim3((unsigned)tiles, (a.rows + rows_a_cta - 1) / rows_a_cta), dim3(i4_join_threads(false)), 0, st, a);
 }

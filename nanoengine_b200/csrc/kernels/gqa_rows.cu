@@ -13,7 +13,7 @@
 // whose quotients are exact or far from a border in 32 bits.  Built without approximate functions.
 //
 // Measured (B200, us, calls in a graph; bytes at 6530 GB/s): 64 / 4 heads of 128 into 4 bits, three axes: 128 tokens 4.6, 4096: 38 (22); 32 / 8 heads into bf16, three axes: 4096: 25 (15);
-// bound there by the chain position, table row, rotation of few resident warps.  4096 rows read back (8 heads): 5.8.  Expanding 32 x 4096 keys of 4 heads: 83 (52).
+// bound there by the chain position, table row, rotation of few resident warps.  4096 rows read back (8 heads): 5.8.  Expanding 32 x 4096 keys of 4 heads: 79 (52).
 #include "kv4.cuh"
 
 namespace ne {

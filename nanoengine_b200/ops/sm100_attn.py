@@ -309,14 +309,14 @@ def _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, sca
     if q.dtype != torch.bfloat16 or q.stride(2) != 1 or q.stride(1) != D or q.stride(0) % 4 or q.data_ptr() % 8:
         q = q.to(torch.bfloat16).clone(memory_format=torch.contiguous_format)
     # Many rows a sequence: unpacking for every 16 of them costs more than expanding the context once.  us of the kernel / of expanding, then the prompt kernel: 32 x 4096 keys,
-    # 64 / 4 heads of 128: 64 rows 92 / 157, 128: 167 / 162, 256: 313 / 172; 16 / 2 heads of 256: 64: 111 / 185, 128: 195 / 182; 16 x 4096, 16 / 2 heads of 64: 256: 56 / 83,
-    # 512: 97 / 92; 4 x 4096, 64 / 4 of 128: 128: 36 / 57, 512: 89 / 75.  The expanded pages take 15 times the room of the 4-bit ones: not where that is more than 2 GB.
+    # 64 / 4 heads of 128: 64 rows 89 / 157, 128: 161 / 157, 256: 301 / 168; 16 / 2 heads of 256: 64: 110 / 185, 128: 192 / 185; 16 x 4096, 16 / 2 heads of 64: 256: 57 / 83,
+    # 512: 98 / 90; 4 x 4096, 64 / 4 of 128: 128: 34 / 57, 512: 87 / 74.  The expanded pages take 15 times the room of the 4-bit ones: not where that is more than 2 GB.
     if (T * g >= (512 if D == 64 else 128) * B and (g % 4 == 0 or g == 1 and Hq % 4 == 0) and g <= 128
             and 4 * B * W * bs * Hkv * D <= _INT4_EXPANDED_BYTES):
         k, v, bt, cl = _k.kv4_expand(k_cache, v_cache, bt, cl, D)
         return gqa_attention_paged(q, k, v, bt, cu, cl, scale, window)
-    # Row tiles of 8 where a sequence has no more rows of a kv head, else of 16.  us of 16 / 8: 128 x 4096 keys, 32 / 8 heads of 128: 159 / 117, of 64: 96 / 77;
-    # 60 x 3000, 16 / 2 heads of 256: 53 / 43.
+    # Row tiles of 8 where a sequence has no more rows of a kv head, else of 16.  us of 16 / 8: 128 x 4096 keys, 32 / 8 heads of 128: 159 / 116, of 64: 96 / 75;
+    # 60 x 3000, 16 / 2 heads of 256: 53 / 41.
     rows = 8 if T * g <= 8 * B else 16
     # equal shares of the batch's work, one for every warp that is resident at once, but no more than its tiles of keys need
     per_sm = _INT4_SHARES.get((D, rows))
