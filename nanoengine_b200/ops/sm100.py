@@ -787,7 +787,7 @@ def gqa_kv_gather(k_cache, v_cache, slots, dim):
     T, hkv = slots.numel(), k_cache.shape[1]
     bs = _kv4_dims(k_cache, v_cache, hkv, dim)
     _same_device(k_cache, v_cache, slots)
-    k, v = torch.empty(2, T, hkv, dim, dtype=torch.bfloat16, device=k_cache.device)
+    k, v = torch.empty(2, T, hkv, dim, dtype=torch.bfloat16, device=k_cache.device).unbind()
     if T:
         _ck(_fn("ne_kv4_gather", "ppplppiiiip")(k_cache.data_ptr(), v_cache.data_ptr(), _i64c(slots).data_ptr(), k_cache.shape[0] * bs, k.data_ptr(), v.data_ptr(), T, hkv, dim,
                                                 bs, _stream()), "ne_kv4_gather")
@@ -821,7 +821,7 @@ def _gqa_rows(qkv, hq, hkv, hd, q_norm_w, k_norm_w, eps, unit_offset, positions,
         if tuple(positions.shape) != (len(sec), T):
             raise ValueError(f"positions {list(positions.shape)}: one row per axis of sections {list(sec)}")
     _same_device(qkv, positions, rope_cache, k_cache, v_cache, slot_mapping, q_norm_w, k_norm_w)
-    q = torch.empty(T, hq, hd, dtype=torch.bfloat16, device=qkv.device)
+    q = qkv.new_empty((T, hq, hd))
     slots = _slots_of(slot_mapping, T)
     if T == 0:
         return q
@@ -831,8 +831,9 @@ def _gqa_rows(qkv, hq, hkv, hd, q_norm_w, k_norm_w, eps, unit_offset, positions,
     for w in (q_norm_w, k_norm_w):
         if w is not None and w.numel() != hd:
             raise ValueError(f"norm weights have {hd} values")
-        w = None if w is None else w.to(torch.bfloat16).contiguous()
-        norms.append(w if w is None or w.data_ptr() % 8 == 0 else w.clone())
+        if w is not None and not (w.dtype == torch.bfloat16 and w.is_contiguous() and w.data_ptr() % 8 == 0):
+            w = w.to(torch.bfloat16).clone(memory_format=torch.contiguous_format)
+        norms.append(w)
     pos = positions if positions.dtype == torch.int64 and positions.stride(-1) == 1 else positions.long().contiguous()
     _ck(_fn("ne_gqa_rows", "pliiippdfplpiipippppliiip")(
         qkv.data_ptr(), qkv.stride(0), hq, hkv, hd, 0 if norms[0] is None else norms[0].data_ptr(), 0 if norms[1] is None else norms[1].data_ptr(), float(eps),

@@ -303,9 +303,9 @@ def _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, sca
     if bt.dim() != 2 or bt.shape[0] < B or cu.numel() != B + 1:
         raise ValueError("one block table row per sequence, and one query boundary more")
     _k._same_device(q, k_cache, v_cache, bt, cu, cl)
-    W, g, dev = bt.shape[1], Hq // Hkv, q.device
+    W, g = bt.shape[1], Hq // Hkv
     if T == 0 or B == 0 or W == 0:
-        return torch.zeros(T, Hq, D, dtype=torch.bfloat16, device=dev)
+        return torch.zeros(T, Hq, D, dtype=torch.bfloat16, device=q.device)
     if q.dtype != torch.bfloat16 or q.stride(2) != 1 or q.stride(1) != D or q.stride(0) % 4 or q.data_ptr() % 8:
         q = q.to(torch.bfloat16).clone(memory_format=torch.contiguous_format)
     # Many rows a sequence: unpacking for every 16 of them costs more than expanding the context once.  us of the kernel / of expanding, then the prompt kernel: 32 x 4096 keys,
@@ -325,9 +325,9 @@ def _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, sca
     tq = rows // g if g < rows else 1
     tiles = min(T, T // tq + B) * Hkv * -(-g // rows)
     shares = min(_sms() * per_sm, -(-tiles * -(-W * bs // (32 if D == 256 else 64)) // 8) * 4)
-    out = torch.empty(T, Hq, D, dtype=torch.bfloat16, device=dev)
-    # partial results, their statistics and the row tiles that cuts run through
-    part = torch.empty(shares * 2 * rows * (D + 1) + 4 * (tiles + 1), dtype=torch.float32, device=dev)
+    out = q.new_empty((T, Hq, D))
+    # partial results, their statistics and the row tiles that cuts run through: 32-bit words, twice as many of q's
+    part = q.new_empty((shares * 4 * rows * (D + 1) + 8 * (tiles + 1),))
     at = part.data_ptr()
     _k._ck(_k._fn("ne_gqa_int4", "plppiipli" + "ppi" + "iiiiiiii" + "f" + "ppppp")(
         q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], bs, bt.data_ptr(), bt.stride(0), W, cu.data_ptr(), cl.data_ptr(), B,
