@@ -12,13 +12,13 @@
 // an element or a scale lies nearer to a border than that (one step of two rows in a hundred), its warp computes it again in 64.  Value rows are bf16,
 // whose quotients are exact or far from a border in 32 bits.  Built without approximate functions.
 //
-// Measured (B200, us, calls in a graph; bytes at 6530 GB/s): 64 / 4 heads of 128 into 4 bits, three axes: 128 tokens 4.6, 4096: 38 (22); 32 / 8 heads into bf16, three axes: 4096: 25 (15);
+// Measured (B200, us, calls in a graph; bytes at 6530 GB/s): 64 / 4 heads of 128 into 4 bits, three axes: 128 tokens 4.4, 4096: 37 (22); 32 / 8 heads into bf16, three axes: 4096: 23 (15);
 // bound there by the chain position, table row, rotation of few resident warps.  4096 rows read back (8 heads): 5.8.  Expanding 32 x 4096 keys of 4 heads: 79 (52).
 #include "kv4.cuh"
 
 namespace ne {
 
-constexpr int kRowsWarps = 8;
+constexpr int kRowsWarps = 4;
 constexpr int kRowsBatch = 4;                         // steps of query rows in flight
 constexpr double kKv4Most = 7 * 1.875 * 32768;       // largest value of the format
 
@@ -223,7 +223,7 @@ __device__ __forceinline__ void split_slot(long long slot, int block_size, long 
 
 // A warp takes `chunk` steps of a token's query heads, or one step of its key heads, or of its value heads; a step is the heads of 32 / L rows.
 template <int L, bool kInt4>
-__global__ void __launch_bounds__(kRowsWarps * 32, 4) gqa_rows_kernel(const RowsArgs a) {
+__global__ void __launch_bounds__(kRowsWarps * 32, 8) gqa_rows_kernel(const RowsArgs a) {
   pdl_wait(); pdl_trigger();
   constexpr int D = 8 * L, R = 32 / L;
   const int lane = threadIdx.x & 31, l = lane % L, sub = lane / L;
@@ -491,7 +491,7 @@ extern "C" int ne_gqa_rows(const void* qkv, long long ld, int Hq, int Hkv, int D
   a.q_out = (__nv_bfloat16*)q_out; a.k_cache = (uint8_t*)k_cache; a.v_cache = (uint8_t*)v_cache; a.slots = slots; a.cache_rows = cache_rows;
   a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.block_size = block_size;
   // Few rows: a warp per step, so that all SMs work; many: several steps under one fetch of the angles.  us of few / many: 64 / 4 heads of 128 into 4 bits, three axes:
-  // 16 tokens 3.3 / 4.2, 128: 5.2 / 4.6, 1024: 27 / 12; 32 / 8 heads: 128: 4.9 / 6.2, 256: 6.5 / 6.9, 512: 9.7 / 8.2; 16 / 2 heads of 256: 128: 4.4 / 4.7, 256: 5.2 / 4.6.
+  // 16 tokens 3.4 / 4.2, 128: 5.3 / 4.6, 1024: 25 / 12; 32 / 8 heads: 128: 4.9 / 5.9, 256: 6.1 / 6.3, 512: 9.5 / 7.4; 16 / 2 heads of 256: 128: 4.6 / 4.4, 256: 5.2 / 4.6.
   const bool many = (long long)T * Hq * D >= 1 << 20;
   a.chunk = many ? 8 : 1;
   a.kv_chunk = many ? 4 : 1;
