@@ -467,6 +467,9 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(const uint8_t* __restri
 using namespace ne;
 
 namespace {
+// The kernels read and write words of eight codes: a head's part of a page has to be whole words (heads of 32: pages of a multiple of 4 tokens, of 64: of 2)
+bool kv4_words(int block_size, int D) { return ((long long)block_size * (D / 2 + D / 32)) % 4 == 0; }
+
 template <int L> int launch_rows(const RowsArgs& a, bool int4, cudaStream_t st) {
   constexpr int R = 32 / L;
   const int q_steps = (a.Hq + R - 1) / R, kv_steps = (a.Hkv + R - 1) / R;
@@ -484,6 +487,7 @@ extern "C" int ne_gqa_rows(const void* qkv, long long ld, int Hq, int Hkv, int D
                            const long long* slots, long long cache_rows, int block_size, int int4, int T, cudaStream_t st) {
   if (T <= 0) return 0;
   if (Hq < 0 || Hkv < 1 || axes < 1 || axes > 4 || max_pos < 1 || block_size < 1) return 1001;
+  if ((int4 && !kv4_words(block_size, D)) || (ld & 3) || ((uintptr_t)qkv & 7) || (((uintptr_t)qw | (uintptr_t)kw) & 7) || ((uintptr_t)rope & 15)) return 1004;
   RowsArgs a{};
   a.qkv = (const __nv_bfloat16*)qkv; a.ld = ld; a.qw = (const __nv_bfloat16*)qw; a.kw = (const __nv_bfloat16*)kw; a.eps = eps; a.w_offset = w_offset;
   a.positions = positions; a.pos_ld = pos_ld; a.rope = rope; a.max_pos = max_pos; a.axes = axes; a.interleaved = interleaved;
@@ -508,6 +512,7 @@ extern "C" int ne_kv4_store(const void* k, const void* v, long long k_ld, long l
                             int Hkv, int D, int block_size, cudaStream_t st) {
   if (T <= 0) return 0;
   if (Hkv < 1 || block_size < 1 || (D != 32 && D != 64 && D != 128 && D != 256)) return 1001;
+  if (!kv4_words(block_size, D) || ((k_ld | v_ld) & 3) || (((uintptr_t)k | (uintptr_t)v) & 7)) return 1004;
   const int per_step = 256 / D, steps = (Hkv + per_step - 1) / per_step;
   const dim3 grid((unsigned)(((long long)T * 2 * steps + kRowsWarps - 1) / kRowsWarps));
   auto go = [&](auto kern) {
@@ -520,7 +525,7 @@ extern "C" int ne_kv4_store(const void* k, const void* v, long long k_ld, long l
 extern "C" int ne_kv4_gather(const void* k_cache, const void* v_cache, const long long* slots, long long cache_rows, void* k_out, void* v_out, int T, int Hkv, int D,
                              int block_size, cudaStream_t st) {
   if (T <= 0) return 0;
-  if (Hkv < 1 || block_size < 1 || D < 32 || D % 32) return 1001;
+  if (Hkv < 1 || block_size < 1 || D < 32 || D % 32 || !kv4_words(block_size, D)) return 1001;
   const long long n = (long long)T * Hkv * (D / 8);
   return (int)launch_pdl(kv4_gather_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, (const uint8_t*)k_cache, (const uint8_t*)v_cache, slots, cache_rows,
                          (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, T, Hkv, D, block_size);
@@ -530,6 +535,7 @@ extern "C" int ne_kv4_gather(const void* k_cache, const void* v_cache, const lon
 extern "C" int ne_kv4_expand(const void* k_cache, const void* v_cache, int num_blocks, const int* tables, long long bt_ld, int bt_width, const int* ctx, int seqs, int width,
                              void* k_out, void* v_out, int* out_tables, int* out_ctx, int Hkv, int D, int block_size, cudaStream_t st) {
   if (seqs <= 0 || width <= 0) return 0;
+  if (!kv4_words(block_size, D)) return 1004;
   if (num_blocks < 1 || Hkv < 1 || block_size < 1 || seqs > 65535 || Hkv > 65535 || (long long)width * 64 < (long long)bt_width * block_size ||
       (long long)seqs * width >= (1ll << 31)) return 1001;
   auto go = [&](auto kern) {

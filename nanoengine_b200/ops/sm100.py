@@ -756,6 +756,8 @@ def _kv4_dims(k_cache, v_cache, hkv: int, dim: int) -> int:
         raise ValueError(f"4-bit keys and values of heads of {dim} come in caches uint8 [blocks, {hkv}, block_size * {row}] of one shape")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()) or (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
         raise ValueError("4-bit caches are contiguous and aligned to 16 bytes")
+    if shape[2] % 4:
+        raise ValueError(f"4-bit rows on the GPU: a head's pages are whole words, not {shape[2]} bytes (head size 32: a multiple of 4 tokens, 64: of 2)")
     return shape[2] // row
 
 
@@ -827,6 +829,8 @@ def _gqa_rows(qkv, hq, hkv, hd, q_norm_w, k_norm_w, eps, unit_offset, positions,
         return q
     if qkv.stride(1) != 1 or qkv.stride(0) % 4 or qkv.data_ptr() % 8:
         qkv = qkv.clone(memory_format=torch.contiguous_format)
+    if rope_cache.data_ptr() % 16:
+        rope_cache = rope_cache.clone()
     norms = []
     for w in (q_norm_w, k_norm_w):
         if w is not None and w.numel() != hd:

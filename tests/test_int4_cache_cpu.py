@@ -241,3 +241,16 @@ def test_step_tables_are_the_host_tables():
     got = ops.step_tables(torch.tensor(new), torch.tensor(ctx), ids, off, bs, sum(new), int(d["max_blocks"]))
     for name in got._fields:
         assert torch.equal(getattr(got, name).flatten().long(), torch.from_numpy(d[name]).flatten().long()), name
+
+
+@pytest.mark.parametrize("dim,bs,fits", [(32, 1, False), (32, 2, False), (32, 3, False), (32, 4, True), (32, 6, False), (64, 1, False), (64, 2, True), (64, 3, False),
+                                         (128, 1, True), (128, 3, True), (256, 1, True)])
+def test_the_gpu_takes_pages_of_whole_words_only(dim, bs, fits):
+    """The kernels move words of eight codes; the check is the host's and needs no GPU."""
+    from nanoengine_b200.ops import sm100
+    cache = torch.zeros(4, 2, ops.kv4_page_bytes(dim, bs), dtype=torch.uint8)
+    if fits:
+        assert sm100._kv4_dims(cache, cache, 2, dim) == bs
+    else:
+        with pytest.raises(ValueError, match="whole words"):
+            sm100._kv4_dims(cache, cache, 2, dim)

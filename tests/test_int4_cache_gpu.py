@@ -213,6 +213,32 @@ def test_rows_of_a_strided_projection():
         assert all(torch.equal(a, b) for a, b in zip(*made))
 
 
+def test_a_rotary_table_at_an_odd_place():
+    g, qkv, qw, kw, pos, table = rows_inputs(7, 8, 2, 128, 1, 3)
+    wide = torch.zeros(table.numel() + 3, device=DEV)
+    made = []
+    for first in (None, 1, 3):
+        if first is not None:
+            wide[first: first + table.numel()] = table.flatten()
+        t = table if first is None else wide[first: first + table.numel()].view_as(table)
+        kc, vc = (torch.zeros(2, 2, ops.kv4_page_bytes(128, 16), dtype=torch.uint8, device=DEV) for _ in range(2))
+        made.append((ops.gqa_qkv_prepare(qkv, 8, 2, 128, qw, kw, 1e-6, False, pos[0], t, kc, vc, torch.arange(7, device=DEV)), kc, vc))
+    for other in made[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(made[0], other))
+
+
+@pytest.mark.parametrize("d,bs", [(32, 4), (32, 12), (64, 2), (64, 6), (128, 1), (128, 3), (256, 1), (256, 5)])
+def test_small_and_odd_pages_of_whole_words(d, bs):
+    T, hkv = 11, 3
+    blocks = T // bs + 2
+    k, v = (torch.randn(T, hkv, d, generator=gen(d + bs)).to(torch.bfloat16).cuda() for _ in range(2))
+    kc, vc = (torch.zeros(blocks, hkv, ops.kv4_page_bytes(d, bs), dtype=torch.uint8, device=DEV) for _ in range(2))
+    slots = torch.randperm(blocks * bs, generator=gen(1))[:T].cuda()
+    ops.gqa_kv_store(kc, vc, slots, k, v)
+    for cache, want, got in zip((kc, vc), (k, v), ops.gqa_kv_gather(kc, vc, slots, d)):
+        assert torch.equal(cache_values(cache, d).flatten(0, 1)[slots], nearest(want)) and torch.equal(got.double(), nearest(want))
+
+
 # ---- attention --------------------------------------------------------------------------------------------------------------------
 ATTENTION = [
     # hq, hkv, dim, block size, new tokens, contexts, window
