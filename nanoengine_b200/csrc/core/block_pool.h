@@ -28,6 +28,19 @@ inline uint64_t chain_hash(uint64_t prev, const int32_t* tok, int n) {
   return h ? h : 1;  // 0 is reserved for "no hash"
 }
 
+// Keys of what a prompt's token ids stand for besides themselves (images, and where their tokens are placed), each mixed into the hash of the block that
+// holds token at[i] and so into those behind it: equal ids that stand for other things never share a page.
+struct PrefixKeys {
+  std::vector<uint64_t> keys;
+  std::vector<int32_t> at;           // ascending
+  uint64_t seed(uint64_t prev, int b, int block_size) const {            // what the hash of block b is chained on
+    const int64_t lo = (int64_t)b * block_size;
+    for (size_t i = 0; i < at.size(); i++)
+      if (at[i] >= lo && at[i] < lo + block_size) prev = mix64(prev ^ keys[i]);
+    return prev;
+  }
+};
+
 class BlockPool {
  public:
   BlockPool() = default;
@@ -55,7 +68,7 @@ class BlockPool {
 
   // Longest cached prefix of `tok`.  Takes a reference on every matched block.
   // At most n-1 tokens count as cached, so the caller always computes one token.
-  std::vector<int32_t> match_prefix(const int32_t* tok, int n, uint64_t* last_hash) {
+  std::vector<int32_t> match_prefix(const int32_t* tok, int n, uint64_t* last_hash, const PrefixKeys& keys = {}) {
     std::vector<int32_t> out;
     *last_hash = 0;
     lookups_++; lookup_tokens_ += (uint64_t)n;
@@ -63,7 +76,7 @@ class BlockPool {
     uint64_t h = 0;
     int max_blocks = (n - 1) / block_size_;
     for (int b = 0; b < max_blocks; b++) {
-      uint64_t nh = chain_hash(h, tok + (size_t)b * block_size_, block_size_);
+      uint64_t nh = chain_hash(keys.seed(h, b, block_size_), tok + (size_t)b * block_size_, block_size_);
       auto it = by_hash_.find(nh);
       if (it == by_hash_.end()) break;
       int id = it->second;

@@ -63,9 +63,11 @@ class Scheduler {
     if (r.prompt_token_ids.empty()) throw std::invalid_argument("empty prompt");
     if (seqs_.count(r.seq_id)) throw std::invalid_argument("duplicate seq_id");
     if ((int)r.prompt_token_ids.size() >= cfg_.max_model_len) throw std::invalid_argument("prompt exceeds max_model_len");
+    if (r.prefix_keys.size() != r.prefix_key_at.size()) throw std::invalid_argument("one place per prefix key");
     auto s = std::make_unique<Sequence>();
     s->seq_id = r.seq_id; s->tokens = r.prompt_token_ids; s->prompt_len = (int)r.prompt_token_ids.size();
     s->sampling = r.sampling_params; s->affinity_key = r.affinity_key; s->vision_slots = r.vision_slots;
+    s->prefix_keys = {r.prefix_keys, r.prefix_key_at};
     s->t_arrival = now_seconds();
     seqs_[r.seq_id] = std::move(s);
     waiting_.push_back(r.seq_id);
@@ -76,7 +78,7 @@ class Scheduler {
   uint64_t add_migration(const RequestMigrate& m) {
     if (seqs_.count(m.seq_id)) throw std::invalid_argument("duplicate seq_id");
     if (m.block_size != cfg_.block_size) throw std::invalid_argument("migration block_size mismatch");
-    if (m.token_ids.empty() || m.prompt_len <= 0 || m.prompt_len > (int)m.token_ids.size())
+    if (m.token_ids.empty() || m.prompt_len <= 0 || m.prompt_len > (int)m.token_ids.size() || m.prefix_keys.size() != m.prefix_key_at.size())
       throw std::invalid_argument("malformed migration request");
     auto s = std::make_unique<Sequence>();
     s->seq_id = m.seq_id; s->tokens = m.token_ids; s->prompt_len = m.prompt_len; s->num_computed = m.num_computed;
@@ -84,6 +86,7 @@ class Scheduler {
     s->pending_migration = false; s->remote_block_table = m.migrate_block_table; s->remote_dp_idx = m.migrate_dp_idx;
     s->remote_handoff_slot = m.migrate_handoff_slot; s->remote_engine_id = m.migrate_engine_id;
     s->remote_state_slot = m.migrate_state_slot;
+    s->prefix_keys = {m.prefix_keys, m.prefix_key_at};
     s->t_arrival = now_seconds(); s->t_first_token = s->t_arrival; s->t_last_token = s->t_arrival;
     seqs_[m.seq_id] = std::move(s);
     waiting_migration_.push_back(m.seq_id);
@@ -407,6 +410,7 @@ class Scheduler {
       m.migrate_block_table = s.block_table; m.migrate_dp_idx = s.dp_idx; m.migrate_state_slot = s.state_slot;
       m.migrate_handoff_slot = s.handoff_slot; m.migrate_hisparse_slot = s.hisparse_slot; m.migrate_engine_id = cfg_.engine_id;
       m.migrate_num_kvcache_blocks = cfg_.num_blocks; m.block_size = cfg_.block_size;
+      m.prefix_keys = s.prefix_keys.keys; m.prefix_key_at = s.prefix_keys.at;
       out.push_back(std::move(m)); exported_.insert(id);
     }
     return out;
@@ -549,7 +553,7 @@ class Scheduler {
     BlockPool& pool = pools_[d];
     int n = (int)s.tokens.size();
     uint64_t h = 0;
-    std::vector<int32_t> matched = pool.match_prefix(s.tokens.data(), n, &h);
+    std::vector<int32_t> matched = pool.match_prefix(s.tokens.data(), n, &h, s.prefix_keys);
     int need = blocks_for(n + spec()) - (int)matched.size();
     std::vector<int32_t> fresh;
     if (need < 0) need = 0;
@@ -675,7 +679,7 @@ class Scheduler {
     BlockPool& pool = pools_[s.dp_idx];
     int full = s.num_computed / cfg_.block_size;
     while (s.commit_cursor < full && s.commit_cursor < (int)s.block_table.size()) {
-      uint64_t h = chain_hash(s.last_block_hash, s.tokens.data() + (size_t)s.commit_cursor * cfg_.block_size, cfg_.block_size);
+      uint64_t h = chain_hash(s.prefix_keys.seed(s.last_block_hash, s.commit_cursor, cfg_.block_size), s.tokens.data() + (size_t)s.commit_cursor * cfg_.block_size, cfg_.block_size);
       pool.commit(s.block_table[s.commit_cursor], h);
       s.last_block_hash = h; s.commit_cursor++;
     }

@@ -9,6 +9,8 @@
 #include <string>
 #include <vector>
 
+#include "block_pool.h"
+
 namespace ne {
 
 struct SamplingParams {
@@ -98,6 +100,7 @@ struct Sequence {
   int32_t prefill_chunks = 0;
   int32_t commit_cursor = 0;         // blocks already published to the prefix cache
   uint64_t last_block_hash = 0;      // chained hash up to commit_cursor
+  PrefixKeys prefix_keys;
   std::vector<float> logprobs;
   std::vector<int32_t> vision_slots;
   // PD migration bookkeeping (decode side)

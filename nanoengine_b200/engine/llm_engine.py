@@ -129,7 +129,8 @@ class LLMEngine:
         """A request whose `image_token_id` prompt tokens stand for image embeddings: given directly ([n, hidden]) or as a slot of
         a vision encoder's pool (`vl.EncoderEngine.encode` + `engine_info()["pool"]`).  The workers splice the rows in during
         prefill.  A model whose rotary positions have several axes places them by the images' patches, `grid_thw` [[t, h, w], ...] (the slot's own when
-        it has them); `spatial_merge_size` patches a side make one token.  Parity: reference engine/llm_component.py:285-340 + runtime/runner/model_runner.py:1557-1573, :1886-1890."""
+        it has them); `spatial_merge_size` patches a side make one token.  The prefix cache shares
+        pages of image tokens, and those behind them, between prompts of the same images at the same places only.  Parity: reference engine/llm_component.py:285-340 + runtime/runner/model_runner.py:1557-1573, :1886-1890."""
         if seq_id is None:
             seq_id = self._next_seq_id
         slot, ntok = (int(vision_slot.slot), int(vision_slot.num_tokens)) if vision_slot is not None else (-1, 0)
@@ -144,7 +145,8 @@ class LLMEngine:
         self._next_seq_id = max(self._next_seq_id, seq_id) + 1
         sp = sampling_params or C.SamplingParams()
         try:
-            return self.scheduler.add_request(C.RequestIn(seq_id, list(prompt_token_ids), sp, 0, [slot] if slot >= 0 else None))
+            at, keys = self.executor.collective_rpc("vision_keys", seq_id)[0] if self.config.enable_prefix_caching else ([], [])
+            return self.scheduler.add_request(C.RequestIn(seq_id, list(prompt_token_ids), sp, 0, [slot] if slot >= 0 else None, keys, at))
         except Exception:
             if axes:
                 self._release_axes(seq_id)

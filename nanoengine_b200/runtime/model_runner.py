@@ -9,6 +9,7 @@ prepare_from_bytes :1829-1948, run_prepared :1984-2132, step timers :84-197; run
 """
 from __future__ import annotations
 
+import hashlib
 import os
 import time
 from typing import Dict, List, Optional
@@ -438,6 +439,21 @@ class ModelRunner:
         self.__dict__.setdefault("_vision", {})[int(seq_id)] = (np.concatenate([[0], np.cumsum(is_img)]), is_img,
                                                                   embeddings.to(self.device, self.dtype))
         return embeddings.shape[0]
+
+    def vision_keys(self, seq_id: int):
+        """(first tokens, keys) of the runs of image tokens of a registered request: a key says in 64 bits what the run stands for, its embeddings as they are
+        spliced in and its positions where it has some of its own."""
+        prefix, is_img, emb = self.__dict__["_vision"][int(seq_id)]
+        own = self._image_axes.get(int(seq_id))
+        edges = np.flatnonzero(np.diff(np.concatenate([[False], is_img, [False]])))
+        rows = emb.contiguous().cpu().view(torch.uint8).numpy()
+        at, keys = edges[::2].tolist(), []
+        for lo, hi in zip(at, edges[1::2].tolist()):
+            h = hashlib.blake2b(rows[int(prefix[lo]): int(prefix[hi])], digest_size=8)
+            if own is not None:
+                h.update(own[0][:, lo: hi].tobytes())
+            keys.append(int.from_bytes(h.digest(), "little"))
+        return at, keys
 
     def release_vision(self, seq_id: int) -> None:
         self.__dict__.get("_vision", {}).pop(int(seq_id), None)
