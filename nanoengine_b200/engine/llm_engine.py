@@ -133,6 +133,8 @@ class LLMEngine:
         pages of image tokens, and those behind them, between prompts of the same images at the same places only.  Parity: reference engine/llm_component.py:285-340 + runtime/runner/model_runner.py:1557-1573, :1886-1890."""
         if seq_id is None:
             seq_id = self._next_seq_id
+        if self.scheduler.get(seq_id) is not None:           # before its images take the place of a live request's
+            raise ValueError("duplicate seq_id")
         slot, ntok = (int(vision_slot.slot), int(vision_slot.num_tokens)) if vision_slot is not None else (-1, 0)
         grids = [list(g) for g in (grid_thw if grid_thw is not None else getattr(vision_slot, "grid_thw", None) or [])]
         axes = bool(grids) and self.config.model_config.position_axes is not None
@@ -148,8 +150,7 @@ class LLMEngine:
             at, keys = self.executor.collective_rpc("vision_keys", seq_id)[0] if self.config.enable_prefix_caching else ([], [])
             return self.scheduler.add_request(C.RequestIn(seq_id, list(prompt_token_ids), sp, 0, [slot] if slot >= 0 else None, keys, at))
         except Exception:
-            if axes:
-                self._release_axes(seq_id)
+            self._release_axes(seq_id)
             raise
 
     # ---- file-backed KV tier ------------------------------------------------------------------

@@ -116,3 +116,19 @@ def test_an_image_in_a_later_turn_keeps_what_the_first_had():
     assert ask(llm, emb, grids, later) == (want, 96)                     # six pages in front of the second image
     assert ask(llm, torch.cat([images(1), images(6)[:4]]), grids, later)[1] == 96
     assert ask(llm, emb, grids, later) == (want, 112)                    # 128 tokens, of which seven full pages count
+
+
+def test_a_refused_request_leaves_the_one_of_its_number_alone():
+    want = ask(make(), images(1), WIDE, seq_id=5)[0]
+    llm = make()
+    llm.engine.add_vision_request(PROMPT, IMG, embeddings=images(1), sampling_params=SP, grid_thw=WIDE, seq_id=5)
+    for grids in (TALL, None):
+        with pytest.raises(ValueError, match="duplicate"):
+            llm.engine.add_vision_request(PROMPT, IMG, embeddings=images(2), sampling_params=SP, grid_thw=grids, seq_id=5)
+    assert llm.generate()[0]["token_ids"] == want
+    llm = make(max_model_len=64)
+    for grids in (WIDE, None):
+        with pytest.raises(ValueError, match="max_model_len"):
+            llm.engine.add_vision_request(PROMPT, IMG, embeddings=images(1), sampling_params=SP, grid_thw=grids)
+    runner = llm.engine.executor.runner
+    assert not runner._vision and not runner._image_axes and not llm.engine._with_axes
