@@ -849,10 +849,13 @@ def _gqa_rows(qkv, hq, hkv, hd, q_norm_w, k_norm_w, eps, unit_offset, positions,
 
 def kv4_expand(k_cache, v_cache, block_tables, context_lens, dim: int):
     """The contexts of all sequences as bf16 caches of 64-token pages of their own: (k, v [B * width, 64, Hkv, dim], block tables [B, width], context lengths).
-    A context is cut off where its block table ends, a page outside the cache reads as zeros."""
+    There are as many sequences as context lengths; tables of more rows are those of a larger batch.  A context is cut off where its block table ends, a page outside the
+    cache reads as zeros."""
     hkv = k_cache.shape[1]
     bs = _kv4_dims(k_cache, v_cache, hkv, dim)
-    B, W = block_tables.shape
+    B, W = context_lens.numel(), block_tables.shape[1]
+    if block_tables.shape[0] < B:
+        raise ValueError(f"{block_tables.shape[0]} block table rows for {B} sequences")
     width = max(1, -(-W * bs // 64))
     k, v = (torch.empty(B * width, 64, hkv, dim, dtype=torch.bfloat16, device=k_cache.device) for _ in range(2))
     bt = torch.empty(B, width, dtype=torch.int32, device=k_cache.device)
