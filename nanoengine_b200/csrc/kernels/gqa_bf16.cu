@@ -108,7 +108,7 @@ gqa_bf16_kernel(const __grid_constant__ CUtensorMap tq_map, const __grid_constan
   const int* bt = a.block_tables;
   if (seq >= 0) {
     const int q_beg = a.cu_seqlens_q[seq], q_len = a.cu_seqlens_q[seq + 1] - q_beg;
-    n_tok = min(a.tq, q_beg + q_len - tok0);
+    n_tok = tok0 < 0 ? 0 : min(a.tq, min(q_beg + q_len, a.T) - tok0);       // boundaries past the last row of q write nothing behind it
     base_limit = a.context_lens[seq] - q_len + (tok0 - q_beg);              // last key visible to the tile's first token
     const int max_limit = base_limit + n_tok - 1;                            // ... to its last token
     const int total_pages = max_limit >= 0 ? max_limit / kGPage + 1 : 0;

@@ -46,3 +46,52 @@ def test_block_tables_of_a_larger_batch(hq, hkv, dim, bs, new, ctx):
     within(got, out, bound)
     with pytest.raises(ValueError, match="block table"):
         ops.gqa_attention_paged(*args[:3], table[: len(ctx) - 1], *args[4:])
+
+
+class Arena:
+    """Hands out the results and workspaces of a call from one patterned buffer, a patterned gap behind each."""
+
+    def __init__(self, monkeypatch, nbytes=256 << 20):
+        self.buf, self.at, self.gaps, self.plain = torch.full((nbytes,), 0xA5, dtype=torch.uint8, device=DEV), 0, [], torch.empty
+        monkeypatch.setattr(torch, "empty", self.empty)
+
+    def empty(self, *size, dtype=None, device=None, **kw):
+        if device is None or torch.device(device).type != "cuda":
+            return self.plain(*size, dtype=dtype, device=device, **kw)
+        size = tuple(size[0]) if len(size) == 1 and not isinstance(size[0], int) else size
+        n = torch.Size(size).numel() * dtype.itemsize
+        lo, self.at = self.at, -(-(self.at + n + 4096) // 512) * 512
+        assert self.at <= self.buf.numel()
+        self.gaps.append((lo + n, self.at))
+        return self.buf[lo: lo + n].view(dtype).view(size)
+
+    def queries(self, q):
+        """q, whose `new_empty` takes from here too."""
+        arena = self
+
+        class Queries(torch.Tensor):
+            def new_empty(self, size, dtype=None):
+                return arena.empty(size, dtype=dtype or self.dtype, device=DEV)
+        return q.as_subclass(Queries)
+
+    def check(self):
+        assert self.gaps and all(bool((self.buf[lo:hi] == 0xA5).all()) for lo, hi in self.gaps)
+
+
+# both prompt kernels over expanded pages, with and without slices of the keys
+@pytest.mark.parametrize("hq,hkv,dim,bs,new,ctx,last", [(64, 4, 128, 64, [70, 33], [70, 200], 150), (64, 4, 128, 64, [16, 17], [2000, 3000], 70), (16, 4, 64, 16, [300], [411], 320), (64, 4, 128, 32, [700, 650], [800, 900], 1351)])
+def test_query_boundaries_past_the_last_row(hq, hkv, dim, bs, new, ctx, last, monkeypatch):
+    """A sequence that claims rows behind the last one of q has its rows where its length puts them, and nothing is written behind a result or a workspace."""
+    args, _, _ = case(hq, hkv, dim, bs, new, ctx, seed=7)
+    T, claimed = sum(new), new[:-1] + [last - sum(new[:-1])]
+    q = torch.full((last + 300, hq, dim), 3.0, dtype=torch.bfloat16, device=DEV)
+    q[:T] = args[0]
+    out, spread, mass, top = dense_attention(q[:last], cache_values(args[1], dim), cache_values(args[2], dim), args[3].cpu(), claimed, ctx, args[6])
+    cu = cu_of(claimed)
+    arena = Arena(monkeypatch)
+    got = ops.gqa_attention_paged(arena.queries(q[:T]), *args[1:4], cu, *args[5:])
+    arena.check()
+    monkeypatch.undo()
+    assert got.untyped_storage().data_ptr() == arena.buf.untyped_storage().data_ptr()
+    within(got, out[:T], attention_bound(out, spread, mass, top)[:T])
+    assert bool((q[T:] == 3).all())
