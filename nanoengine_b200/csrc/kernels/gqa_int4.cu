@@ -66,12 +66,12 @@ struct I4Seq { int q_beg, q_len, ctx, first, per_tile, tiles; };        // first
 template <int KEYS> __device__ __forceinline__ I4Seq i4_seq(const I4Args& a, int q_beg, int q_end, int ctx) {
   I4Seq s;
   s.q_beg = q_beg;
-  s.q_len = min(max(0, q_end - q_beg), a.T);
+  s.q_len = max(0, q_end - q_beg);                                       // (as claimed: it says where the rows stand, also where some lie behind the last one of q)
   s.ctx = (int)max(0ll, min((long long)ctx, (long long)a.bt_width * a.block_size));
   const int first_key = a.window > 0 ? max(0, s.ctx - s.q_len - a.window + 1) : 0;
   s.first = first_key / KEYS;
   s.per_tile = max(1, (s.ctx + KEYS - 1) / KEYS - s.first);              // a tile that sees no key still writes its zeros
-  s.tiles = (s.q_len + a.tq - 1) / a.tq;
+  s.tiles = (min(s.q_len, max(0, a.T - max(q_beg, 0))) + a.tq - 1) / a.tq;
   return s;
 }
 template <int KEYS> __device__ __forceinline__ I4Seq i4_load(const I4Args& a, int i) {

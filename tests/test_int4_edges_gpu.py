@@ -78,8 +78,9 @@ class Arena:
         assert self.gaps and all(bool((self.buf[lo:hi] == 0xA5).all()) for lo, hi in self.gaps)
 
 
-# both prompt kernels over expanded pages, with and without slices of the keys
-@pytest.mark.parametrize("hq,hkv,dim,bs,new,ctx,last", [(64, 4, 128, 64, [70, 33], [70, 200], 150), (64, 4, 128, 64, [16, 17], [2000, 3000], 70), (16, 4, 64, 16, [300], [411], 320), (64, 4, 128, 32, [700, 650], [800, 900], 1351)])
+# the kernel that reads 4-bit pages (8 and 16 rows), then both prompt kernels over expanded pages, with and without slices of the keys
+@pytest.mark.parametrize("hq,hkv,dim,bs,new,ctx,last", [(8, 2, 128, 64, [1, 2], [90, 300], 40), (64, 4, 128, 64, [1, 3], [90, 300], 9), (64, 4, 128, 64, [70, 33], [70, 200], 150),
+                                                        (64, 4, 128, 64, [16, 17], [2000, 3000], 70), (16, 4, 64, 16, [300], [411], 320), (64, 4, 128, 32, [700, 650], [800, 900], 1351)])
 def test_query_boundaries_past_the_last_row(hq, hkv, dim, bs, new, ctx, last, monkeypatch):
     """A sequence that claims rows behind the last one of q has its rows where its length puts them, and nothing is written behind a result or a workspace."""
     args, _, _ = case(hq, hkv, dim, bs, new, ctx, seed=7)
