@@ -618,6 +618,8 @@ def _check_step_out(out, sizes) -> None:
         want = torch.int64 if name in ("positions", "slot_mapping") else torch.int32
         if o.dtype != want or o.dim() != len(size) or any(have < need for have, need in zip(o.shape, size)) or (o.numel() and o.stride(-1) != 1):
             raise ValueError(f"step_tables: out.{name} must be {want} of at least {list(size)} with unit inner stride")
+        if len(size) == 2 and size[0] > 1 and o.stride(0) < size[1]:
+            raise ValueError(f"step_tables: the rows of out.{name} overlap")
 
 
 # ---- pooled rows --------------------------------------------------------------------------------------------

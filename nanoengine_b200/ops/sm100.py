@@ -894,7 +894,7 @@ def step_tables(q_lens, seq_lens, block_ids, block_offsets, block_size, num_toke
         ref._check_step_out(out, sizes)
         _same_device(*out)
         cu, ctx, pos, slot, table, last = (o[tuple(slice(k) for k in size)] for o, size in zip(out, sizes))
-        ld = max(table.stride(0), max_blocks)
+        ld = table.stride(0) if rows > 1 else max_blocks
     _ck(_fn("ne_step_tables", "pppp" + "iiiiiiii" + "ppppp" + "lpp")(
         q_lens.data_ptr(), seq_lens.data_ptr(), block_ids.data_ptr(), block_offsets.data_ptr(), B, rows, n_ids, block_size, num_tokens, max_blocks, pad_len, scratch_block,
         cu.data_ptr(), ctx.data_ptr(), pos.data_ptr(), slot.data_ptr(), table.data_ptr(), ld, last.data_ptr(), _stream()), "ne_step_tables")

@@ -1,0 +1,24 @@
+"""4-bit pages, positions on several axes and step tables: calls at the edges of what the operators allow."""
+import pytest
+import torch
+
+from nanoengine_b200 import ops
+
+
+def overlapping(device):
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32, device=device)                 # noqa: E731
+    i64 = lambda n: torch.zeros(n, dtype=torch.int64, device=device)                 # noqa: E731
+    new, ctx, ids, off = (torch.tensor(t, dtype=torch.int32, device=device) for t in ([1, 1], [5, 40], [3, 1, 2], [0, 1, 3]))
+    for table in (i32(4).expand(2, 4), i32(6).as_strided((2, 4), (1, 1)), i32(2).expand(2, 2)):
+        out = ops.StepTables(i32(3), i32(2), i64(2), i64(2), table, i32(2))
+        with pytest.raises(ValueError, match="overlap"):
+            ops.step_tables(new, ctx, ids, off, 32, 2, 2, out=out)
+        assert not table.any()
+    # one row may have any stride
+    out = ops.StepTables(i32(2), i32(1), i64(1), i64(1), i32(4).expand(1, 4), i32(1))
+    got = ops.step_tables(new[:1], ctx[1:], ids[1:], off[:2] * 2, 32, 1, 2, out=out)
+    assert got.block_tables.tolist() == [[1, 2]] and got.slot_mapping.tolist() == [71]
+
+
+def test_tables_whose_rows_overlap_are_refused():
+    overlapping("cpu")

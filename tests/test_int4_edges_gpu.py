@@ -96,3 +96,8 @@ def test_query_boundaries_past_the_last_row(hq, hkv, dim, bs, new, ctx, last, mo
     assert got.untyped_storage().data_ptr() == arena.buf.untyped_storage().data_ptr()
     within(got, out[:T], attention_bound(out, spread, mass, top)[:T])
     assert bool((q[T:] == 3).all())
+
+
+def test_tables_whose_rows_overlap_are_refused():
+    from test_int4_edges_cpu import overlapping
+    overlapping(DEV)
