@@ -690,9 +690,13 @@ def gqa_qkv_prepare(qkv, hq, hkv, hd, q_norm_w, k_norm_w, eps, unit_offset, posi
                     interleaved=False):
     """One kernel for head split, q / k RMSNorm, rotary embedding and the paged K / V store (head dim 128 or 256 with the whole
     head rotated, bf16 caches); other shapes run the same steps as separate kernels.  Positions on several axes and 4-bit caches: one
-    kernel for head dims 32, 64, 128 and 256."""
+    kernel for head dims 32, 64, 128 and 256; several axes over bf16 caches at other head dims: the separate kernels."""
     T = qkv.shape[0]
-    if sections is not None or k_cache.dtype == torch.uint8:
+    if sections is not None and k_cache.dtype != torch.uint8 and hd not in KV4_DIMS:
+        if T == 0:
+            return qkv.new_empty((0, hq, hd))
+        rope_cache, positions = _axes_table(positions, rope_cache, sections, interleaved, T, hd), torch.arange(T, device=qkv.device)
+    elif sections is not None or k_cache.dtype == torch.uint8:
         return _gqa_rows(qkv, hq, hkv, hd, q_norm_w, k_norm_w, eps, unit_offset, positions, rope_cache, k_cache, v_cache, slot_mapping, sections, interleaved)
     fused = (hd in (128, 256) and rope_cache.shape[1] == hd and qkv.dtype == torch.bfloat16 and qkv.stride(1) == 1 and qkv.stride(0) % 2 == 0
              and k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16 and k_cache.is_contiguous() and v_cache.is_contiguous()
@@ -796,6 +800,31 @@ def gqa_kv_gather(k_cache, v_cache, slots, dim):
     return k, v
 
 
+def _sections(sections, positions, T: int, hd: int):
+    sec = tuple(int(n) for n in sections)
+    if sum(sec) != hd // 2 or min(sec) < 0 or not 1 <= len(sec) <= 4:
+        raise ValueError(f"sections {list(sec)}: one to four axes whose angles add up to half a head, {hd // 2}")
+    if tuple(positions.shape) != (len(sec), T):
+        raise ValueError(f"positions {list(positions.shape)}: one row per axis of sections {list(sec)}")
+    return sec
+
+
+def _axes_table(positions, rope_cache, sections, interleaved: bool, T: int, hd: int):
+    """Every token's own row of cosines and sines [T, hd], its angles at the positions of their axes (never outside the table).  Nothing comes from the host: it can be captured."""
+    if rope_cache.dtype != torch.float32 or rope_cache.dim() != 2 or rope_cache.shape[1] != hd:
+        raise ValueError(f"the rotary table is fp32 [positions, {hd}]")
+    sec = _sections(sections, positions, T, hd)
+    i = torch.arange(hd // 2, device=rope_cache.device)
+    axis = torch.zeros_like(i)
+    for a in range(1, len(sec)):
+        if interleaved:
+            axis += a * ((i % len(sec) == a) & (i < len(sec) * sec[a]))
+        else:
+            axis += i >= sum(sec[:a])
+    place = positions.long().clamp(0, rope_cache.shape[0] - 1).t()[:, axis]
+    return torch.cat([rope_cache[place, i], rope_cache[place, i + hd // 2]], -1)
+
+
 def _gqa_rows(qkv, hq, hkv, hd, q_norm_w, k_norm_w, eps, unit_offset, positions, rope_cache, k_cache, v_cache, slot_mapping, sections, interleaved):
     T = qkv.shape[0]
     int4 = k_cache.dtype == torch.uint8
@@ -817,11 +846,7 @@ def _gqa_rows(qkv, hq, hkv, hd, q_norm_w, k_norm_w, eps, unit_offset, positions,
         if positions.numel() != T:
             raise ValueError(f"{positions.numel()} positions for {T} tokens")
     else:
-        sec = tuple(int(n) for n in sections)
-        if sum(sec) != hd // 2 or min(sec) < 0 or not 1 <= len(sec) <= 4:
-            raise ValueError(f"sections {list(sec)}: one to four axes whose angles add up to half a head, {hd // 2}")
-        if tuple(positions.shape) != (len(sec), T):
-            raise ValueError(f"positions {list(positions.shape)}: one row per axis of sections {list(sec)}")
+        sec = _sections(sections, positions, T, hd)
     _same_device(qkv, positions, rope_cache, k_cache, v_cache, slot_mapping, q_norm_w, k_norm_w)
     q = qkv.new_empty((T, hq, hd))
     slots = _slots_of(slot_mapping, T)

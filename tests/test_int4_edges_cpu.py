@@ -22,3 +22,16 @@ def overlapping(device):
 
 def test_tables_whose_rows_overlap_are_refused():
     overlapping("cpu")
+
+
+@pytest.mark.parametrize("sections,interleaved", [([48], False), ([16, 16, 16], True), ([20, 0, 28], False), ([24, 16, 8], True), ([10, 12, 14, 12], False), ([4, 30, 7, 7], True)])
+def test_rows_of_angles_by_axis(sections, interleaved):
+    """What the GPU's separate kernels turn rows by is the plain form's table."""
+    from nanoengine_b200.ops import reference as ref, sm100
+    g = torch.Generator().manual_seed(1)
+    table, pos = torch.randn(50, 96, generator=g), torch.randint(0, 50, (len(sections), 9), generator=g)
+    assert torch.equal(sm100._axes_table(pos, table, sections, interleaved, 9, 96), ref.rope_axes_rows(pos, table, sections, interleaved))
+    with pytest.raises(ValueError, match="sections"):
+        sm100._axes_table(pos, table, [47], interleaved, 9, 96)
+    with pytest.raises(ValueError, match="one row per axis"):
+        sm100._axes_table(pos[:, :8], table, sections, interleaved, 9, 96)

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from int4_cases import attention_bound, cache_values, dense_attention, random_cache, softmax_scale, table_of
+from int4_cases import BF16_HALF_STEP, attention_bound, cache_values, dense_attention, random_cache, rope_table, rows_exact, softmax_scale, table_of
 from nanoengine_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -101,3 +101,61 @@ def test_query_boundaries_past_the_last_row(hq, hkv, dim, bs, new, ctx, last, mo
 def test_tables_whose_rows_overlap_are_refused():
     from test_int4_edges_cpu import overlapping
     overlapping(DEV)
+
+
+@pytest.mark.parametrize("T,hq,hkv,d,sections,interleaved,norm", [(1, 4, 1, 96, [16, 16, 16], True, True), (37, 8, 2, 80, [8, 20, 12], False, True),
+                                                                   (130, 4, 4, 112, [24, 16, 16], True, False), (5, 8, 2, 96, [0, 48], False, True)])
+def test_several_axes_at_other_head_sizes(T, hq, hkv, d, sections, interleaved, norm):
+    """Head sizes that the row kernel is not built for, bf16 caches: norm and rotation are rounded one behind the other, as with one position."""
+    g = gen(d)
+    qkv = torch.randn(T, (hq + 2 * hkv) * d, generator=g).to(torch.bfloat16).cuda()
+    qw, kw = ((1 + 0.2 * torch.randn(d, generator=g)).to(torch.bfloat16).cuda() if norm else None for _ in range(2))
+    table, pos = rope_table(d, 500, DEV), torch.randint(0, 500, (len(sections), T), generator=g).cuda()
+    kc, vc = (torch.full((T // 16 + 2, 16, hkv, d), 3.0, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    slots = torch.randperm(kc.shape[0] * 16, generator=g)[:T].cuda()
+    x = qkv.view(T, -1, d).clone()
+    call = lambda: ops.gqa_qkv_prepare(qkv, hq, hkv, d, qw, kw, 1e-6, False, pos, table, kc, vc, slots, sections, interleaved)       # noqa: E731
+    q = call()
+    # two roundings: of the normed row (either element of a pair, turned by at most 1 each) and of the result
+    h = BF16_HALF_STEP * (2 if norm else 1) * (1 + 2.0 ** -7)
+    for got, rows, w in ((q, x[:, :hq], qw), (kc.flatten(0, 1)[slots], x[:, hq: hq + hkv], kw)):
+        want = rows_exact(rows, w, 1e-6, 0.0, pos, table, sections, interleaved)
+        size = rows_exact(rows, w, 1e-6, 0.0, torch.zeros_like(pos), table, sections, interleaved)       # normed, not turned
+        a, b = size.chunk(2, -1)
+        pair = (a.abs() + b.abs()).repeat(1, 1, 2)
+        assert bool(((got.double() - want).abs() <= h * pair + 2.0 ** -18 * pair.amax(-1, keepdim=True)).all())
+    assert torch.equal(vc.flatten(0, 1)[slots], x[:, hq + hkv:])
+    # equal positions on all axes are ordinary positions, to the bit
+    one = pos[:1].expand(len(sections), T)
+    kc2, kc3, vc2 = kc.clone(), kc.clone(), vc.clone()
+    a = ops.gqa_qkv_prepare(x.view(T, -1).clone(), hq, hkv, d, qw, kw, 1e-6, False, one, table, kc2, vc2, slots, sections, interleaved)
+    b = ops.gqa_qkv_prepare(x.view(T, -1).clone(), hq, hkv, d, qw, kw, 1e-6, False, pos[0], table, kc3, vc2, slots)
+    assert torch.equal(a, b) and torch.equal(kc2, kc3)
+    # positions past the table stay inside it, and the call can be captured
+    far = pos.clone()
+    far[0, 0], far[-1, -1] = 10 ** 12, -5
+    qkv.copy_(x.view(T, -1))
+    want = ops.gqa_qkv_prepare(x.view(T, -1).clone(), hq, hkv, d, qw, kw, 1e-6, False, far.clamp(0, 499), table, kc2, vc2, slots, sections, interleaved)
+    pos.copy_(far)
+    call()
+    qkv.copy_(x.view(T, -1))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    qkv.copy_(x.view(T, -1))
+    graph.replay()
+    assert torch.equal(got, want) and torch.equal(kc.flatten(0, 1)[slots], kc2.flatten(0, 1)[slots])
+
+
+def test_an_engine_with_three_axes_and_heads_of_96():
+    from nanoengine_b200 import Config, LLM, SamplingParams
+    from nanoengine_b200.models.config import ModelConfig
+    sp, ps = SamplingParams(temperature=0.0, max_tokens=8, ignore_eos=True), [list(range(3, 60)), list(range(100, 117))]
+    got = []
+    for over in (dict(), dict(mrope_section=[16, 16, 16], mrope_interleaved=True)):
+        mc = ModelConfig(architecture="Qwen3MoeForCausalLM", vocab_size=512, hidden_size=256, num_hidden_layers=2, num_attention_heads=8, num_key_value_heads=2, head_dim=96,
+                         intermediate_size=512, n_routed_experts=0, first_k_dense_replace=0, q_lora_rank=None, rope_theta=1e6, max_position_embeddings=4096, qk_norm=True,
+                         eos_token_id=None, **over)
+        llm = LLM(Config(model="small", model_config=mc, dummy_weight=True, device="cuda", kvcache_block_size=64, max_num_seqs=4, num_kvcache_blocks=32, max_model_len=256, seed=0))
+        got.append([o["token_ids"] for o in sorted(llm.generate(ps, sp), key=lambda o: o["seq_id"])])
+    assert got[0] == got[1]                       # text: the same position on every axis
