@@ -863,7 +863,8 @@ def _gqa_rows(qkv, hq, hkv, hd, q_norm_w, k_norm_w, eps, unit_offset, positions,
         if w is not None and not (w.dtype == torch.bfloat16 and w.is_contiguous() and w.data_ptr() % 8 == 0):
             w = w.to(torch.bfloat16).clone(memory_format=torch.contiguous_format)
         norms.append(w)
-    pos = positions if positions.dtype == torch.int64 and positions.stride(-1) == 1 else positions.long().contiguous()
+    # one position a token: in a row, whatever its shape (a column of a wider tensor has a last stride of 1 too); several axes: rows of them, any distance apart
+    pos = _i64c(positions) if sections is None else positions if positions.dtype == torch.int64 and positions.stride(1) == 1 else positions.long().contiguous()
     _ck(_fn("ne_gqa_rows", "pliiippdfplpiipippppliiip")(
         qkv.data_ptr(), qkv.stride(0), hq, hkv, hd, 0 if norms[0] is None else norms[0].data_ptr(), 0 if norms[1] is None else norms[1].data_ptr(), float(eps),
         1.0 if unit_offset else 0.0, pos.data_ptr(), pos.stride(0) if sections is not None else 0, rope_cache.data_ptr(), rope_cache.shape[0], len(sec),

@@ -159,3 +159,21 @@ def test_an_engine_with_three_axes_and_heads_of_96():
         llm = LLM(Config(model="small", model_config=mc, dummy_weight=True, device="cuda", kvcache_block_size=64, max_num_seqs=4, num_kvcache_blocks=32, max_model_len=256, seed=0))
         got.append([o["token_ids"] for o in sorted(llm.generate(ps, sp), key=lambda o: o["seq_id"])])
     assert got[0] == got[1]                       # text: the same position on every axis
+
+
+def test_positions_in_a_column_of_a_wider_tensor():
+    T, d = 12, 64
+    g = gen(3)
+    qkv = torch.randn(T, 4 * d, generator=g).to(torch.bfloat16).cuda()
+    table, wide = rope_table(d, 99, DEV), torch.randint(0, 99, (T, 3), generator=g).cuda()
+    made = []
+    for pos in (wide[:, 1].contiguous(), wide[:, 1:2], wide[:, 1], wide[:, 1].int()):
+        kc, vc = (torch.zeros(1, 1, ops.kv4_page_bytes(d, 16), dtype=torch.uint8, device=DEV) for _ in range(2))
+        made.append((ops.gqa_qkv_prepare(qkv, 2, 1, d, None, None, 1e-6, False, pos, table, kc, vc, torch.arange(T, device=DEV)), kc))
+    assert all(torch.equal(q, made[0][0]) and torch.equal(kc, made[0][1]) for q, kc in made)
+    three = [wide.t(), wide.t().contiguous(), torch.cat([wide, wide], 1).t()[:3], wide.t().int()]           # rows of axes with any strides
+    made = []
+    for pos in three:
+        kc, vc = (torch.zeros(1, 1, ops.kv4_page_bytes(d, 16), dtype=torch.uint8, device=DEV) for _ in range(2))
+        made.append((ops.gqa_qkv_prepare(qkv, 2, 1, d, None, None, 1e-6, False, pos, table, kc, vc, torch.arange(T, device=DEV), [8, 12, 12]), kc))
+    assert all(torch.equal(q, made[0][0]) and torch.equal(kc, made[0][1]) for q, kc in made)
