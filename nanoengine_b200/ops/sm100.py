@@ -858,10 +858,10 @@ def _gqa_rows(qkv, hq, hkv, hd, q_norm_w, k_norm_w, eps, unit_offset, positions,
         rope_cache = rope_cache.clone()
     norms = []
     for w in (q_norm_w, k_norm_w):
-        if w is not None and w.numel() != hd:
-            raise ValueError(f"norm weights have {hd} values")
-        if w is not None and not (w.dtype == torch.bfloat16 and w.is_contiguous() and w.data_ptr() % 8 == 0):
-            w = w.to(torch.bfloat16).clone(memory_format=torch.contiguous_format)
+        if w is not None and (w.numel() != hd or w.dtype != torch.bfloat16):          # the kernel reads bf16: wider ones would lose bits unseen
+            raise ValueError(f"norm weights are {hd} bf16 values, not {w.numel()} of {w.dtype}")
+        if w is not None and not (w.is_contiguous() and w.data_ptr() % 8 == 0):
+            w = w.clone(memory_format=torch.contiguous_format)
         norms.append(w)
     # one position a token: in a row, whatever its shape (a column of a wider tensor has a last stride of 1 too); several axes: rows of them, any distance apart
     pos = _i64c(positions) if sections is None else positions if positions.dtype == torch.int64 and positions.stride(1) == 1 else positions.long().contiguous()

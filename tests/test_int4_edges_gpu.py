@@ -177,3 +177,17 @@ def test_positions_in_a_column_of_a_wider_tensor():
         kc, vc = (torch.zeros(1, 1, ops.kv4_page_bytes(d, 16), dtype=torch.uint8, device=DEV) for _ in range(2))
         made.append((ops.gqa_qkv_prepare(qkv, 2, 1, d, None, None, 1e-6, False, pos, table, kc, vc, torch.arange(T, device=DEV), [8, 12, 12]), kc))
     assert all(torch.equal(q, made[0][0]) and torch.equal(kc, made[0][1]) for q, kc in made)
+
+
+@pytest.mark.parametrize("sections", [None, [8, 12, 12]])
+def test_norm_weights_that_bf16_does_not_hold_are_refused(sections):
+    """The plain form takes them as they are (1 + 2^-9 is 1 in bf16); the kernel has no form for them."""
+    T, d = 4, 64
+    qkv = torch.randn(T, 4 * d, generator=gen(1)).to(torch.bfloat16).cuda()
+    pos, table = torch.zeros(3 if sections else 1, T, dtype=torch.long, device=DEV), rope_table(d, 9, DEV)
+    kc = torch.zeros(1, 1, ops.kv4_page_bytes(d, 16), dtype=torch.uint8, device=DEV)
+    good, odd = torch.ones(d, dtype=torch.bfloat16, device=DEV), torch.ones(d, device=DEV) + 2.0 ** -9
+    for qw, kw in ((odd, good), (good, odd), (good[:32], good)):
+        with pytest.raises(ValueError, match="norm weights"):
+            ops.gqa_qkv_prepare(qkv, 2, 1, d, qw, kw, 1e-6, False, pos if sections else pos[0], table, kc, kc.clone(), torch.arange(T, device=DEV), sections)
+    assert not kc.any()
