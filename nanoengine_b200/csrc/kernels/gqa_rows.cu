@@ -66,16 +66,17 @@ template <int L, typename R> __device__ __forceinline__ void norm_and_turn(R (&x
   for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   const R mean = ss / (R)(8 * L) + eps, r = norm ? rsqrt(mean) : (R)1;
   const bool lost = norm && !(mean > (R)1e-30 && mean < (R)1e37);        // squares that 32 bits do not hold: no bound
-  // Error in 32 bits, relative to the sum of the two magnitudes: 7 2^-24 of the mean (14 additions, halved by the root), 2^-22 of the root, 2^-24 each for
-  // weight, factor, two products, sum and scaling: below 2^-20
+  // Error in 32 bits, relative to the sum of the two magnitudes, in units of 2^-24: 8 of the mean (a product, 13 additions, eps rounded and added: 16, halved by the
+  // root), 4 of the root (two units in the last place), one each for the weight, its factor, the product, the sum and the scaling: 17.  20 are taken: the rest
+  // is for the products of errors and for the roundings of `off` itself
 #pragma unroll
   for (int e = 0; e < 4; e++) {
     const R a = x[e], b = x[4 + e];
     x[e] = r * (a * t.ca[e] - b * t.sb[e]);
     x[4 + e] = r * (b * t.cb[e] + a * t.sa[e]);
     if (off) {
-      off[e] = lost ? INFINITY : (float)(r * (fabs(a * t.ca[e]) + fabs(b * t.sb[e]))) * 0x1p-20f;
-      off[4 + e] = lost ? INFINITY : (float)(r * (fabs(b * t.cb[e]) + fabs(a * t.sa[e]))) * 0x1p-20f;
+      off[e] = lost ? INFINITY : (float)(r * (fabs(a * t.ca[e]) + fabs(b * t.sb[e]))) * 0x1.4p-20f;
+      off[4 + e] = lost ? INFINITY : (float)(r * (fabs(b * t.cb[e]) + fabs(a * t.sa[e]))) * 0x1.4p-20f;
     }
   }
 }

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from int4_cases import BF16_HALF_STEP, attention_bound, cache_values, dense_attention, random_cache, rope_table, rows_exact, softmax_scale, table_of
+from int4_cases import BF16_HALF_STEP, attention_bound, cache_values, dense_attention, nearest, random_cache, rope_table, rows_exact, softmax_scale, table_of
 from nanoengine_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -191,3 +191,18 @@ def test_norm_weights_that_bf16_does_not_hold_are_refused(sections):
         with pytest.raises(ValueError, match="norm weights"):
             ops.gqa_qkv_prepare(qkv, 2, 1, d, qw, kw, 1e-6, False, pos if sections else pos[0], table, kc, kc.clone(), torch.arange(T, device=DEV), sections)
     assert not kc.any()
+
+
+@pytest.mark.parametrize("d,T", [(64, 40000), (128, 40000), (256, 20000)])
+def test_codes_of_many_key_rows_are_those_of_64_bits(d, T):
+    """Ten million elements a size: some lie nearer to a border than the 32-bit error allows to tell."""
+    g = torch.Generator(device=DEV).manual_seed(d)
+    hkv, bs = 4, 64
+    qkv = torch.randn(T, 3 * hkv * d, generator=g, device=DEV).to(torch.bfloat16)
+    kw = (1 + 0.2 * torch.randn(d, generator=g, device=DEV)).to(torch.bfloat16)
+    pos, table = torch.randint(0, 4000, (3, T), generator=g, device=DEV), rope_table(d, 4000, DEV)
+    kc, vc = (torch.zeros(-(-T // bs), hkv, ops.kv4_page_bytes(d, bs), dtype=torch.uint8, device=DEV) for _ in range(2))
+    sec = [d // 4, d // 8, d // 8]
+    ops.gqa_qkv_prepare(qkv, hkv, hkv, d, kw, kw, 1e-6, True, pos, table, kc, vc, torch.arange(T, device=DEV), sec, True)
+    want = nearest(rows_exact(qkv.view(T, -1, d)[:, hkv: 2 * hkv], kw, 1e-6, 1.0, pos, table, sec, True))
+    assert torch.equal(cache_values(kc, d).flatten(0, 1)[:T], want)
