@@ -60,6 +60,7 @@ struct FmArgs {
   const __nv_bfloat16* q; const __nv_bfloat16* k; const __nv_bfloat16* v; const __nv_bfloat16* k_rope;
   long long q_ld, k_ld, v_ld, r_ld;            // k_ld, v_ld: from one token to the next (pages too)
   int d, k_dim;
+  int own_pages;                               // pages of a cache that the call brings with it, 0: those of the engine's (the bounds-checked build compares with them)
 };
 
 // (x, y) <- (x, y) scale + shift, and sum += (x, y): two fp32 operations in one instruction
@@ -117,7 +118,7 @@ __device__ __forceinline__ void fmha_row_again(const FmArgs& a, const int* bt, i
   auto token = [&](int key) -> long long {   // row of the key, -1: of a page that is none
     if (!a.paged) return k_beg + key;
     const int page = bt[key / kFmBlk];
-    return NE_INDEX_OK(page, BK_CACHE_PAGES, kKernelFm, __LINE__) ? (long long)page * kFmBlk + key % kFmBlk : -1;
+    return NE_PAGE_OK(page, a.own_pages, kKernelFm, __LINE__) ? (long long)page * kFmBlk + key % kFmBlk : -1;
   };
 #pragma unroll 1
   for (int key0 = inv > 0.f ? lo : hi + 1; key0 <= hi; key0 += 32) {
@@ -249,7 +250,7 @@ fmha_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         int page = 0;
         if (a.paged) {
           page = bt[blk0 + j];
-          if (!NE_INDEX_OK(page, BK_CACHE_PAGES, kKernelFm, __LINE__)) page = 0;
+          if (!NE_PAGE_OK(page, a.own_pages, kKernelFm, __LINE__)) page = 0;
         }
         const int n = v ? a.nv : a.nc;
         for (; room < n; tail++) {
@@ -415,7 +416,7 @@ fmha_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
           if (key0 + i > limit || key0 + i < lowest) r[i] = 0xff800000u;
       }
 #ifdef NE_DEBUG_BOUNDS
-      if (a.paged && !NE_INDEX_OK(a.block_tables[(long long)seq * a.bt_stride + blk0 + j], BK_CACHE_PAGES, kKernelFm, __LINE__)) {      // keys of a page that is none
+      if (a.paged && !NE_PAGE_OK(a.block_tables[(long long)seq * a.bt_stride + blk0 + j], a.own_pages, kKernelFm, __LINE__)) {      // keys of a page that is none
 #pragma unroll
         for (int i = 0; i < 64; i++) r[i] = 0xff800000u;
       }
@@ -562,7 +563,7 @@ using namespace ne;
 // q [T, Hq, D] with row stride q_ld (elements; heads D apart), keys / values either pages k, v [num_blocks, 64, Hkv, D or Dv] contiguous (block_tables
 // not null) or rows [T, Hkv, D or Dv] with row strides k_ld, v_ld; k_rope not null (ragged only): the last D - Dk_nope columns of every head's key are the
 // row k_rope [T, D - Dk_nope] (row stride r_ld), k_nope heads k_head apart.  context_lens null: keys are the sequence's own tokens.
-// split_p: probabilities as two bf16 terms.  splits > 1: part / lse2 as ne_attn_merge takes them.
+// split_p: bit 0: probabilities as two bf16 terms, bit 1: the pages are the call's own, not the engine's.  splits > 1: part / lse2 as ne_attn_merge takes them.
 extern "C" int ne_fmha(const void* q, long long q_ld, const void* k, long long k_ld, int k_dim, const void* k_rope, long long r_ld, const void* v, long long v_ld,
                        int num_blocks, const int* block_tables, int bt_stride, const int* cu_seqlens_q, const int* context_lens, int num_seqs, int T, int Hq,
                        int Hkv, int D, int Dv, int tiles, int grid_x, int splits, int window, int causal, float scale, int split_p, void* out, float* part,
@@ -585,6 +586,8 @@ extern "C" int ne_fmha(const void* q, long long q_ld, const void* k, long long k
   a.block_tables = block_tables; a.bt_stride = bt_stride; a.cu_seqlens_q = cu_seqlens_q; a.context_lens = context_lens; a.num_seqs = num_seqs;
   a.scale_log2 = scale * 1.4426950408889634f; a.out = (__nv_bfloat16*)out; a.part = part; a.lse2 = lse2;
   a.q = (const __nv_bfloat16*)q; a.k = (const __nv_bfloat16*)k; a.v = (const __nv_bfloat16*)v; a.k_rope = (const __nv_bfloat16*)k_rope;
+  a.own_pages = split_p & 2 ? num_blocks : 0;
+  split_p &= 1;
   a.d = D; a.k_dim = k_rope ? k_dim : D; a.q_ld = q_ld; a.r_ld = r_ld; a.k_ld = a.paged ? (long long)Hkv * D : k_ld; a.v_ld = a.paged ? (long long)Hkv * Dv : v_ld;
   CUtensorMap mq, mk, mv, mr;
   {

@@ -40,6 +40,7 @@ struct GqaArgs {
   float scale_log2;
   __nv_bfloat16* out;                        // [T, Hq, 128] (splits == 1)
   float* part; float* lse2;                  // [splits, T, Hq, 128], [splits, T, Hq] (splits > 1)
+  int own_pages;                             // pages of a cache that the call brings with it, 0: those of the engine's
 };
 
 __global__ void __launch_bounds__(kGqaThreads, 1)
@@ -129,7 +130,7 @@ gqa_bf16_kernel(const __grid_constant__ CUtensorMap tq_map, const __grid_constan
         uint8_t* dst = sKV + s * kStage;
         mbar_expect_tx(b_kvfull + 8 * s, kStage);
         int block = bt[pg_begin + i];
-        if (!NE_INDEX_OK(block, BK_CACHE_PAGES, 7, __LINE__)) block = 0;      // a bad page id reads page 0 instead of another allocation
+        if (!NE_PAGE_OK(block, a.own_pages, 7, __LINE__)) block = 0;      // a bad page id reads page 0 instead of another allocation
         tma_load_5d(smem_u32(dst), &tk_map, b_kvfull + 8 * s, 0, 0, hkv, block, 0);
         tma_load_5d(smem_u32(dst + kGKBytes), &tv_map, b_kvfull + 8 * s, 0, 0, hkv, block, 0);
       }
@@ -324,7 +325,7 @@ using namespace ne;
 // sum over sequences of ceil(q_len / (128 / g)) known on the host (e.g. T for decode, ceil(T / tq) + num_seqs in general).
 extern "C" int ne_gqa_bf16(const void* q, const void* k_cache, const void* v_cache, int num_blocks, const int* block_tables, int bt_stride,
                            const int* cu_seqlens_q, const int* context_lens, int num_seqs, int T, int Hq, int Hkv, int max_tiles, int splits,
-                           float scale, void* out, float* part, float* lse2, cudaStream_t st) {
+                           float scale, int own_pages, void* out, float* part, float* lse2, cudaStream_t st) {
   if (T <= 0) return 0;
   if (Hkv < 1 || Hq % Hkv || splits < 1 || (splits > 1 && (!part || !lse2))) return 1001;
   const int g = Hq / Hkv;
@@ -352,7 +353,7 @@ extern "C" int ne_gqa_bf16(const void* q, const void* k_cache, const void* v_cac
   GqaArgs a;
   a.block_tables = block_tables; a.bt_stride = bt_stride; a.cu_seqlens_q = cu_seqlens_q; a.context_lens = context_lens; a.num_seqs = num_seqs;
   a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.g = g; a.tq = tq; a.splits = splits; a.scale_log2 = scale * 1.4426950408889634f;
-  a.out = (__nv_bfloat16*)out; a.part = part; a.lse2 = lse2;
+  a.out = (__nv_bfloat16*)out; a.part = part; a.lse2 = lse2; a.own_pages = own_pages;
   return (int)launch_pdl(gqa_bf16_kernel, dim3(dim3((unsigned)max_tiles, (unsigned)Hkv, (unsigned)splits)), dim3(kGqaThreads), kGqaSmem,
                          st, mq, mk, mv, a);
 }

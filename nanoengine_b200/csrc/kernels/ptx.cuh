@@ -35,15 +35,18 @@ __device__ __forceinline__ void report(int code, int kernel_id, int a, int b) {
 enum BoundKind : int { BK_CACHE_ROWS = 0, BK_CACHE_PAGES = 1, BK_STATE_SLOTS = 2, BK_EXPERTS = 3, BK_COUNT = 4 };
 #ifdef NE_DEBUG_BOUNDS
 extern __device__ long long g_bounds[BK_COUNT];
-__device__ __forceinline__ bool ne_index_ok(long long idx, int kind, int kernel_id, int site) {
-  const long long n = g_bounds[kind];
+__device__ __forceinline__ bool ne_index_ok(long long idx, int kind, int kernel_id, int site, long long own = 0) {
+  const long long n = own > 0 ? own : g_bounds[kind];
   if (n <= 0 || (idx >= 0 && idx < n)) return true;        // no bound registered: nothing to compare with
   report(ST_BAD_INDEX, kernel_id, site, (int)idx);
   return false;
 }
 #define NE_INDEX_OK(idx, kind, kernel_id, site) ne_index_ok((long long)(idx), kind, kernel_id, site)
+// a page of a call whose pages are its own (pages of a temporary cache) where own > 0, else of the registered cache
+#define NE_PAGE_OK(idx, own, kernel_id, site) ne_index_ok((long long)(idx), BK_CACHE_PAGES, kernel_id, site, own)
 #else
 #define NE_INDEX_OK(idx, kind, kernel_id, site) true
+#define NE_PAGE_OK(idx, own, kernel_id, site) true
 #endif
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }

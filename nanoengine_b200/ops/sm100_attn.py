@@ -193,7 +193,7 @@ def _fmha_tiles(T: int, B: int, Hq: int, Hkv: int, D: int, Dv: int) -> int:
     return 1 if Dv > 128 or D > 192 or T < B * tq or min(T, T // tq + B) * Hkv <= _sms() else 2
 
 
-def _fmha(q, k, v, cu, scale, causal, split_p, block_tables=None, context_lens=None, window=0, k_rope=None):
+def _fmha(q, k, v, cu, scale, causal, split_p, block_tables=None, context_lens=None, window=0, k_rope=None, own_pages=False):
     """The tcgen05 prompt kernel, for sizes that `_fmha_covers`; rows and pages as the kernel's entry wants them."""
     T, Hq, D = q.shape
     paged = block_tables is not None
@@ -214,7 +214,7 @@ def _fmha(q, k, v, cu, scale, causal, split_p, block_tables=None, context_lens=N
     at = lambda t: 0 if t is None else t.data_ptr()          # noqa: E731
     _k._ck(_fmha_call()(q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), k.shape[-1], at(k_rope), 0 if k_rope is None else k_rope.stride(0), v.data_ptr(),
                         v.stride(0), k.shape[0], at(block_tables), block_tables.stride(0) if paged else 0, cu.data_ptr(), at(context_lens), B, T, Hq, Hkv, D, Dv,
-                        tiles, grid, S, max(0, int(window)), 1 if causal else 0, scale, 1 if split_p else 0, out.data_ptr(), at(part), at(lse2),
+                        tiles, grid, S, max(0, int(window)), 1 if causal else 0, scale, (1 if split_p else 0) | (2 if own_pages else 0), out.data_ptr(), at(part), at(lse2),
                         torch.cuda.current_stream().cuda_stream), "ne_fmha")
     PROMPT_TC_CALLS[0] += 1
     if S > 1:
@@ -231,9 +231,14 @@ def _rows16(t):
 def gqa_attention_paged(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale, window: int = 0):
     """`window` > 0: every query sees only its last `window` key positions (sliding-window layers).  bf16 caches of 64-token pages: tensor cores.  Those
     layers, and head sizes other than 128, keep their probabilities in 32-bit (two bf16 terms); other caches run on the generic kernel."""
-    T, Hq, D = q.shape
     if k_cache.dtype == torch.uint8:
         return _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale, window)
+    return _gqa_pages(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale, window)
+
+
+def _gqa_pages(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale, window, own_pages=False):
+    """`own_pages`: the caches were made for this call, the bound that is registered for the engine's pages is not theirs."""
+    T, Hq, D = q.shape
     Hkv = k_cache.shape[2]
     lib = _k.lib()
     bt, cu, cl = _i32(block_tables), _i32(cu_seqlens_q), _i32(context_lens)
@@ -251,7 +256,7 @@ def gqa_attention_paged(q, k_cache, v_cache, block_tables, cu_seqlens_q, context
         # this, 64 / 4 heads: 4 prompts of 1000: 183 / 138, one of 600 (304 tiles): 26 / 20; 8 / 1 heads, one of 2000 (126 tiles): 31 / 38; 128 x 2 tokens: 150 / 172
         tq = 128 // group
         if T >= B * tq and min(T, T // tq + B) * Hkv > _sms():
-            return _fmha(q, k_cache, v_cache, cu, scale, True, False, bt, cl)
+            return _fmha(q, k_cache, v_cache, cu, scale, True, False, bt, cl, own_pages=own_pages)
         out = torch.empty(T, Hq, D, dtype=torch.bfloat16, device=q.device)
         # tcgen05 kernel: one CTA per (kv head, tile of 128 (token, head) rows, key slice)
         max_tiles = min(T, T // tq + B)
@@ -264,7 +269,7 @@ def gqa_attention_paged(q, k_cache, v_cache, block_tables, cu_seqlens_q, context
             lse2 = torch.empty(S, T, Hq, dtype=torch.float32, device=q.device)
         _k._ck(lib.ne_gqa_bf16(_k._p(q), _k._p(k_cache), _k._p(v_cache), _c.c_int(k_cache.shape[0]), _k._p(bt), _c.c_int(bt.stride(0)), _k._p(cu),
                                _k._p(cl), _c.c_int(B), _c.c_int(T), _c.c_int(Hq), _c.c_int(Hkv), _c.c_int(max_tiles), _c.c_int(S), _c.c_float(scale),
-                               _k._p(out), _k._p(part), _k._p(lse2), _k._st()), "ne_gqa_bf16")
+                               _c.c_int(k_cache.shape[0] if own_pages else 0), _k._p(out), _k._p(part), _k._p(lse2), _k._st()), "ne_gqa_bf16")
         if S > 1:
             _k._ck(lib.ne_attn_merge(_k._p(part), _k._p(lse2), _k._p(out), _c.c_int(S), _c.c_longlong(T * Hq), _c.c_int(D), _c.c_int(D), _k._st()),
                    "ne_attn_merge")
@@ -272,7 +277,7 @@ def gqa_attention_paged(q, k_cache, v_cache, block_tables, cu_seqlens_q, context
     assert group % 4 == 0 or group == 1 and Hq % 4 == 0 or Hkv == Hq, "query heads per kv head must be a multiple of 4"
     if (pages64 and scale > 0 and _fmha_covers(group, D, D) and k_cache.shape[3] == v_cache.shape[3] == D and k_cache.data_ptr() % 16 == 0
             and v_cache.data_ptr() % 16 == 0):
-        return _fmha(q if _rows16(q) else q.clone(memory_format=torch.contiguous_format), k_cache, v_cache, cu, scale, True, True, bt, cl, window)
+        return _fmha(q if _rows16(q) else q.clone(memory_format=torch.contiguous_format), k_cache, v_cache, cu, scale, True, True, bt, cl, window, own_pages=own_pages)
     out = torch.empty(T, Hq, D, dtype=torch.bfloat16, device=q.device)
     _k._ck(lib.ne_attn_generic(_k._p(q), _c.c_longlong(q.stride(0)), _c.c_int(q.stride(1)), _k._p(k_cache), _k._p(v_cache),
                                _c.c_longlong(Hkv * D), _c.c_int(D), _c.c_int(group), _k._p(bt), _c.c_int(bt.stride(0)), _c.c_int(k_cache.shape[1]),
@@ -314,7 +319,7 @@ def _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, sca
     if (T * g >= (512 if D == 64 else 128) * B and (g % 4 == 0 or g == 1 and Hq % 4 == 0) and g <= 128
             and 4 * B * W * bs * Hkv * D <= _INT4_EXPANDED_BYTES):
         k, v, bt, cl = _k.kv4_expand(k_cache, v_cache, bt, cl, D)
-        return gqa_attention_paged(q, k, v, bt, cu, cl, scale, window)
+        return _gqa_pages(q, k, v, bt, cu, cl, scale, window, own_pages=True)
     # Row tiles of 8 where a sequence has no more rows of a kv head, else of 16.  us of 16 / 8: 128 x 4096 keys, 32 / 8 heads of 128: 159 / 116, of 64: 96 / 75;
     # 60 x 3000, 16 / 2 heads of 256: 53 / 41.
     rows = 8 if T * g <= 8 * B else 16
