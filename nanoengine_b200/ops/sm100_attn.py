@@ -292,6 +292,28 @@ _INT4_SHARES = {}
 _INT4_EXPANDED_BYTES = 2 << 30       # what a step over 4-bit pages may take for pages in bf16
 
 
+def _int4_expanded_bytes(B: int, W: int, Hkv: int, D: int, bs: int) -> int:
+    """Bytes of both caches of expanded pages for B sequences under block tables W wide."""
+    return 4 * B * max(1, -(-W * bs // 64)) * 64 * Hkv * D
+
+
+def _int4_min_rows(Hq: int, Hkv: int, D: int) -> int:
+    """Rows (tokens times heads of a group) a sequence, in the mean, from which a step runs over pages expanded to bf16; 0: never.
+    Unpacking for every 16 rows then costs more than expanding the context once.  us of the kernel / of expanding, then the prompt kernel: 32 x 4096 keys, 64 / 4 heads of 128:
+    64 rows 89 / 157, 128: 161 / 157, 256: 301 / 168; 16 / 2 heads of 256: 64: 110 / 185, 128: 192 / 185; 16 x 4096, 16 / 2 heads of 64: 256: 57 / 83, 512: 98 / 90;
+    4 x 4096, 64 / 4 of 128: 128: 34 / 57, 512: 87 / 74."""
+    g = Hq // Hkv
+    return (512 if D == 64 else 128) if (g % 4 == 0 or g == 1 and Hq % 4 == 0) and g <= 128 else 0
+
+
+def int4_expansion_room(max_tokens: int, max_seqs: int, max_len: int, Hq: int, Hkv: int, D: int, bs: int) -> int:
+    """The most bytes that the expanded pages of one step can take (a layer's go before the next layer's come): what an engine over 4-bit pages leaves free beside
+    its cache."""
+    rows = _int4_min_rows(Hq, Hkv, D)
+    seqs = min(max_seqs, max_tokens * (Hq // Hkv) // rows) if rows else 0
+    return min(_INT4_EXPANDED_BYTES, _int4_expanded_bytes(seqs, -(-max_len // bs) + 1, Hkv, D, bs)) if seqs else 0
+
+
 def _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale, window: int):
     """4-bit pages: a kernel that unpacks them in registers for steps of few query rows per key, the tensor-core kernels over pages expanded to bf16 for others."""
     T, Hq, D = q.shape
@@ -313,11 +335,9 @@ def _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, sca
         return torch.zeros(T, Hq, D, dtype=torch.bfloat16, device=q.device)
     if q.dtype != torch.bfloat16 or q.stride(2) != 1 or q.stride(1) != D or q.stride(0) % 4 or q.data_ptr() % 8:
         q = q.to(torch.bfloat16).clone(memory_format=torch.contiguous_format)
-    # Many rows a sequence: unpacking for every 16 of them costs more than expanding the context once.  us of the kernel / of expanding, then the prompt kernel: 32 x 4096 keys,
-    # 64 / 4 heads of 128: 64 rows 89 / 157, 128: 161 / 157, 256: 301 / 168; 16 / 2 heads of 256: 64: 110 / 185, 128: 192 / 185; 16 x 4096, 16 / 2 heads of 64: 256: 57 / 83,
-    # 512: 98 / 90; 4 x 4096, 64 / 4 of 128: 128: 34 / 57, 512: 87 / 74.  The expanded pages take 15 times the room of the 4-bit ones: not where that is more than 2 GB.
-    if (T * g >= (512 if D == 64 else 128) * B and (g % 4 == 0 or g == 1 and Hq % 4 == 0) and g <= 128
-            and 4 * B * W * bs * Hkv * D <= _INT4_EXPANDED_BYTES):
+    # many rows a sequence; the expanded pages take 64 / 17 times the room of the 4-bit ones: not where that is more than 2 GB
+    many = _int4_min_rows(Hq, Hkv, D)
+    if many and T * g >= many * B and _int4_expanded_bytes(B, W, Hkv, D, bs) <= _INT4_EXPANDED_BYTES:
         k, v, bt, cl = _k.kv4_expand(k_cache, v_cache, bt, cl, D)
         return _gqa_pages(q, k, v, bt, cu, cl, scale, window, own_pages=True)
     # Row tiles of 8 where a sequence has no more rows of a kv head, else of 16.  us of 16 / 8: 128 x 4096 keys, 32 / 8 heads of 128: 159 / 116, of 64: 96 / 75;

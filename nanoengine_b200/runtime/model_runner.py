@@ -247,10 +247,20 @@ class ModelRunner:
         used = total - free
         torch.cuda.empty_cache()
         blocks = kv_budget_blocks(self.plan, total, self.config.gpu_memory_utilization, used, peak, current,
-                                  reserved=self.plan.state_bytes + self.plan.hisparse_device_bytes)
+                                  reserved=self.plan.state_bytes + self.plan.hisparse_device_bytes + self._expansion_bytes())
         if self.plan.hisparse:      # the cold tier is bounded by the pinned host memory it may take
             blocks = min(blocks, int(self.config.hisparse_host_gb * (1 << 30)) // max(1, self.plan.kv_block_bytes))
         return blocks
+
+    def _expansion_bytes(self) -> int:
+        """Room for the bf16 pages that prompts over a 4-bit cache run on: a portion behind a long context takes more of them than the warm-up's prompt, which has
+        nothing in front of it."""
+        if not self.plan.int4:
+            return 0
+        from ..ops.sm100_attn import int4_expansion_room
+        c = self.config
+        return int4_expansion_room(c.max_num_batched_tokens, c.max_num_seqs, c.max_model_len, self.mc.num_attention_heads // c.attention_tp, self.plan.kv_heads_local,
+                                   self.plan.row_dim, self.plan.block_size)
 
     def _warmup_prefill(self, tokens: int) -> None:
         bs = self.plan.block_size

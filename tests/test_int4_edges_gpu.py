@@ -206,3 +206,29 @@ def test_codes_of_many_key_rows_are_those_of_64_bits(d, T):
     ops.gqa_qkv_prepare(qkv, hkv, hkv, d, kw, kw, 1e-6, True, pos, table, kc, vc, torch.arange(T, device=DEV), sec, True)
     want = nearest(rows_exact(qkv.view(T, -1, d)[:, hkv: 2 * hkv], kw, 1e-6, 1.0, pos, table, sec, True))
     assert torch.equal(cache_values(kc, d).flatten(0, 1)[:T], want)
+
+
+@pytest.mark.parametrize("kv", ["int4", "auto"])
+def test_the_room_of_expanded_pages_stays_outside_the_cache(kv, monkeypatch):
+    """A cache sized from free memory leaves what the widest prompt step over it expands."""
+    from nanoengine_b200 import Config, LLM, SamplingParams
+    from nanoengine_b200.models.config import ModelConfig
+    from nanoengine_b200.ops import sm100_attn
+    from nanoengine_b200.runtime import model_runner
+    seen, plain = [], model_runner.kv_budget_blocks
+
+    def budget(*a, reserved=0, **kw):
+        seen.append(reserved)
+        return min(300, plain(*a, reserved=reserved, **kw))
+
+    monkeypatch.setattr(model_runner, "kv_budget_blocks", budget)
+    mc = ModelConfig(architecture="Qwen3MoeForCausalLM", vocab_size=512, hidden_size=256, num_hidden_layers=2, num_attention_heads=8, num_key_value_heads=2, head_dim=128,
+                     intermediate_size=512, n_routed_experts=0, first_k_dense_replace=0, q_lora_rank=None, rope_theta=1e6, max_position_embeddings=8192, qk_norm=True,
+                     eos_token_id=None)
+    llm = LLM(Config(model="small", model_config=mc, dummy_weight=True, device="cuda", kv_cache_dtype=kv, kvcache_block_size=64, max_num_seqs=4, max_num_batched_tokens=1024,
+                     max_model_len=4096, gpu_memory_utilization=0.2, enforce_eager=True, seed=0))
+    assert seen == [sm100_attn.int4_expansion_room(1024, 4, 4096, 8, 2, 128, 64) if kv == "int4" else 0]
+    # a portion of 1000 tokens behind 3000: no more than that is taken beside the cache
+    sp = SamplingParams(temperature=0.0, max_tokens=1, ignore_eos=True)
+    llm.generate([[5 + i % 400 for i in range(3900)]], sp)
+    assert kv == "auto" or seen[0] >= 4 * 3904 * 2 * 128
