@@ -85,7 +85,7 @@ class LLMEngine:
         self.scheduler = C.Scheduler(build_scheduler_config(config, self.num_blocks, plan.plan_bits()))
         self.executor.collective_rpc("allocate_kvcache", self.num_blocks)
         self._next_seq_id = 1
-        self._with_axes = set()        # requests whose workers keep image positions for them
+        self._with_axes = set()        # requests whose workers keep images, or image positions, for them
         self.migrator = None   # set by the PD layer (disagg.KVMigrator)
         self.endpoint = None   # ZMQ endpoint of the engine process serving this engine, once it has one (published with the description)
         self._pd_connect = None        # connector of a prefill engine found through the control plane (tests substitute it)
@@ -142,8 +142,7 @@ class LLMEngine:
             raise ValueError("image positions on several axes stay with the worker that ran the prompt: use mode='hybrid'")
         self.executor.collective_rpc("register_vision", seq_id, list(prompt_token_ids), int(image_token_id), embeddings, pool_desc, slot, ntok,
                                      grids if axes else None, int(spatial_merge_size))
-        if axes:
-            self._with_axes.add(seq_id)
+        self._with_axes.add(seq_id)
         self._next_seq_id = max(self._next_seq_id, seq_id) + 1
         sp = sampling_params or C.SamplingParams()
         try:
@@ -220,7 +219,7 @@ class LLMEngine:
         step_outs = self.scheduler.postprocess_runner_out_bytes(outs, ms)
         if self._with_axes:
             for o in step_outs:
-                if o.seq_id in self._with_axes and o.status == C.FINISHED:
+                if o.seq_id in self._with_axes and o.status in (C.FINISHED, C.TO_BE_MIGRATED):
                     self._release_axes(o.seq_id)
         if self.l3_enabled:
             self._l3_persist()

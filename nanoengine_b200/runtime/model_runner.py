@@ -446,17 +446,18 @@ class ModelRunner:
         if grid_thw and self.position_axes is not None:
             from ..vl.positions import image_positions
             self._image_axes[int(seq_id)] = image_positions(is_img, grid_thw, merge)
-        self.__dict__.setdefault("_vision", {})[int(seq_id)] = (np.concatenate([[0], np.cumsum(is_img)]), is_img,
-                                                                  embeddings.to(self.device, self.dtype))
+        # the rows on the device until the prompt is in, on the host until the request ends: a preempted prompt starts over with them
+        rows = embeddings.to(self.device, self.dtype)
+        self.__dict__.setdefault("_vision", {})[int(seq_id)] = [np.concatenate([[0], np.cumsum(is_img)]), is_img, rows, rows.cpu()]
         return embeddings.shape[0]
 
     def vision_keys(self, seq_id: int):
         """(first tokens, keys) of the runs of image tokens of a registered request: a key says in 64 bits what the run stands for, its embeddings as they are
         spliced in and its positions where it has some of its own."""
-        prefix, is_img, emb = self.__dict__["_vision"][int(seq_id)]
+        prefix, is_img, _, host = self.__dict__["_vision"][int(seq_id)]
         own = self._image_axes.get(int(seq_id))
         edges = np.flatnonzero(np.diff(np.concatenate([[False], is_img, [False]])))
-        rows = emb.contiguous().cpu().view(torch.uint8).numpy()
+        rows = host.contiguous().view(torch.uint8).numpy()
         at, keys = edges[::2].tolist(), []
         for lo, hi in zip(at, edges[1::2].tolist()):
             h = hashlib.blake2b(rows[int(prefix[lo]): int(prefix[hi])], digest_size=8)
@@ -481,15 +482,17 @@ class ModelRunner:
         for sid, q, n in zip(b.seq_ids, b.q_lens, b.seq_lens):
             ent = reg.get(int(sid))
             if ent is not None:
-                prefix, is_img, emb = ent
+                prefix, is_img, emb, host = ent
                 lo, hi = n - q, min(n, len(is_img))                     # prompt positions covered by this chunk
                 if hi > lo:
                     sel = np.nonzero(is_img[lo:hi])[0]
                     if sel.size:
+                        if emb is None:
+                            emb = ent[2] = host.to(x.device)
                         rows = torch.from_numpy(sel + row).to(x.device)
                         x.index_copy_(0, rows, emb[int(prefix[lo]): int(prefix[lo]) + sel.size])
                 if n >= len(is_img):
-                    reg.pop(int(sid))                                   # the whole prompt is in: the rows are no longer needed
+                    ent[2] = None                                       # the whole prompt is in
             row += q
         return x
 

@@ -132,3 +132,21 @@ def test_a_refused_request_leaves_the_one_of_its_number_alone():
             llm.engine.add_vision_request(PROMPT, IMG, embeddings=images(1), sampling_params=SP, grid_thw=grids)
     runner = llm.engine.executor.runner
     assert not runner._vision and not runner._image_axes and not llm.engine._with_axes
+
+
+@pytest.mark.parametrize("axes", [True, False])
+@pytest.mark.parametrize("kw", [dict(enable_prefix_caching=False), dict(), dict(max_num_batched_tokens=112)])
+def test_preempted_prompts_are_computed_again_with_their_images(axes, kw):
+    """Without a host tier a preempted prompt starts over: its image rows have to be there again."""
+    grids = [WIDE, TALL] if axes else [None, None]
+    want = [ask(make(enable_prefix_caching=False), images(i + 1), g)[0] for i, g in enumerate(grids)]
+    llm = make(num_kvcache_blocks=14, **kw)                              # room for two prompts of seven pages, not for the answers
+    for i, g in enumerate(grids):
+        llm.engine.add_vision_request(PROMPT, IMG, embeddings=images(i + 1), sampling_params=SP, grid_thw=g, seq_id=i + 1)
+    preempted, out, runner = 0, {1: [], 2: []}, llm.engine.executor.runner
+    while not llm.engine.is_finished():
+        for o in llm.engine.step():
+            out[o.seq_id] += o.token_ids
+        preempted += sum(v.num_preemptions for v in map(llm.engine.scheduler.get, (1, 2)) if v is not None)
+    assert preempted and [out[1], out[2]] == want
+    assert not runner._vision and not runner._image_axes and not llm.engine._with_axes
