@@ -120,15 +120,15 @@ PYBIND11_MODULE(_core, m) {
 
   py::class_<RequestIn>(m, "RequestIn")
       .def(py::init([](uint64_t seq_id, std::vector<int32_t> prompt, SamplingParams sp, uint64_t affinity, py::object vision,
-                       std::vector<uint64_t> prefix_keys, std::vector<int32_t> prefix_key_at) {
+                       std::vector<uint64_t> prefix_keys, std::vector<int32_t> prefix_key_at, int32_t position_shift) {
              RequestIn r; r.seq_id = seq_id; r.prompt_token_ids = std::move(prompt); r.sampling_params = sp; r.affinity_key = affinity;
              if (!vision.is_none()) r.vision_slots = vision.cast<std::vector<int32_t>>();
-             r.prefix_keys = std::move(prefix_keys); r.prefix_key_at = std::move(prefix_key_at);
+             r.prefix_keys = std::move(prefix_keys); r.prefix_key_at = std::move(prefix_key_at); r.position_shift = position_shift;
              return r;
            }),
            py::arg("seq_id"), py::arg("prompt_token_ids"), py::arg("sampling_params") = SamplingParams{},
            py::arg("affinity_key") = 0, py::arg("vision_slots") = py::none(),
-           py::arg("prefix_keys") = std::vector<uint64_t>{}, py::arg("prefix_key_at") = std::vector<int32_t>{})
+           py::arg("prefix_keys") = std::vector<uint64_t>{}, py::arg("prefix_key_at") = std::vector<int32_t>{}, py::arg("position_shift") = 0)
       .def_readwrite("seq_id", &RequestIn::seq_id)
       .def_readwrite("prompt_token_ids", &RequestIn::prompt_token_ids)
       .def_readwrite("sampling_params", &RequestIn::sampling_params)
@@ -136,6 +136,7 @@ PYBIND11_MODULE(_core, m) {
       .def_readwrite("vision_slots", &RequestIn::vision_slots)
       .def_readwrite("prefix_keys", &RequestIn::prefix_keys)
       .def_readwrite("prefix_key_at", &RequestIn::prefix_key_at)
+      .def_readwrite("position_shift", &RequestIn::position_shift)
       .def("to_bytes", [](const RequestIn& r) { return py::bytes(r.to_bytes()); })
       .def_static("from_bytes", [](const std::string& b) { return RequestIn::from_bytes(b); });
 
@@ -158,6 +159,7 @@ PYBIND11_MODULE(_core, m) {
       .def_readwrite("block_size", &RequestMigrate::block_size)
       .def_readwrite("prefix_keys", &RequestMigrate::prefix_keys)
       .def_readwrite("prefix_key_at", &RequestMigrate::prefix_key_at)
+      .def_readwrite("position_shift", &RequestMigrate::position_shift)
       .def_property_readonly("metadata", [](const RequestMigrate& r) { return py::make_tuple(r.seq_id, r.first_token()); })
       .def("to_bytes", [](const RequestMigrate& r) { return py::bytes(r.to_bytes()); })
       .def_static("from_bytes", [](const std::string& b) { return RequestMigrate::from_bytes(b); });
@@ -293,6 +295,7 @@ PYBIND11_MODULE(_core, m) {
       .def_readonly("status", &Sequence::status)
       .def_readonly("dp_idx", &Sequence::dp_idx)
       .def_readonly("block_table", &Sequence::block_table)
+      .def_readonly("position_shift", &Sequence::position_shift)
       .def_readonly("host_blocks", &Sequence::host_blocks)
       .def_readonly("state_slot", &Sequence::state_slot)
       .def_readonly("handoff_slot", &Sequence::handoff_slot)

@@ -67,7 +67,7 @@ class Scheduler {
     auto s = std::make_unique<Sequence>();
     s->seq_id = r.seq_id; s->tokens = r.prompt_token_ids; s->prompt_len = (int)r.prompt_token_ids.size();
     s->sampling = r.sampling_params; s->affinity_key = r.affinity_key; s->vision_slots = r.vision_slots;
-    s->prefix_keys = {r.prefix_keys, r.prefix_key_at};
+    s->prefix_keys = {r.prefix_keys, r.prefix_key_at}; s->position_shift = r.position_shift;
     s->t_arrival = now_seconds();
     seqs_[r.seq_id] = std::move(s);
     waiting_.push_back(r.seq_id);
@@ -86,7 +86,7 @@ class Scheduler {
     s->pending_migration = false; s->remote_block_table = m.migrate_block_table; s->remote_dp_idx = m.migrate_dp_idx;
     s->remote_handoff_slot = m.migrate_handoff_slot; s->remote_engine_id = m.migrate_engine_id;
     s->remote_state_slot = m.migrate_state_slot;
-    s->prefix_keys = {m.prefix_keys, m.prefix_key_at};
+    s->prefix_keys = {m.prefix_keys, m.prefix_key_at}; s->position_shift = m.position_shift;
     s->t_arrival = now_seconds(); s->t_first_token = s->t_arrival; s->t_last_token = s->t_arrival;
     seqs_[m.seq_id] = std::move(s);
     waiting_migration_.push_back(m.seq_id);
@@ -410,7 +410,7 @@ class Scheduler {
       m.migrate_block_table = s.block_table; m.migrate_dp_idx = s.dp_idx; m.migrate_state_slot = s.state_slot;
       m.migrate_handoff_slot = s.handoff_slot; m.migrate_hisparse_slot = s.hisparse_slot; m.migrate_engine_id = cfg_.engine_id;
       m.migrate_num_kvcache_blocks = cfg_.num_blocks; m.block_size = cfg_.block_size;
-      m.prefix_keys = s.prefix_keys.keys; m.prefix_key_at = s.prefix_keys.at;
+      m.prefix_keys = s.prefix_keys.keys; m.prefix_key_at = s.prefix_keys.at; m.position_shift = s.position_shift;
       out.push_back(std::move(m)); exported_.insert(id);
     }
     return out;

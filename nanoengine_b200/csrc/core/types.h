@@ -101,6 +101,7 @@ struct Sequence {
   int32_t commit_cursor = 0;         // blocks already published to the prefix cache
   uint64_t last_block_hash = 0;      // chained hash up to commit_cursor
   PrefixKeys prefix_keys;
+  int32_t position_shift = 0;        // behind the prompt a token at index i stands at i + shift (images take fewer positions than tokens)
   std::vector<float> logprobs;
   std::vector<int32_t> vision_slots;
   // PD migration bookkeeping (decode side)

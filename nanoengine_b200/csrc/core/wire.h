@@ -118,15 +118,16 @@ struct RequestIn {
   std::vector<int32_t> vision_slots;
   std::vector<uint64_t> prefix_keys;   // what the prompt's token ids from prefix_key_at[i] on stand for besides themselves
   std::vector<int32_t> prefix_key_at;
+  int32_t position_shift = 0;
   std::string to_bytes() const {
     ByteWriter w; w.header(TAG_REQUEST_IN); w.u64(seq_id); w.vec(prompt_token_ids);
     write_sampling(w, sampling_params); w.u64(affinity_key); w.vec(vision_slots);
-    w.vec(prefix_keys); w.vec(prefix_key_at); return w.buf;
+    w.vec(prefix_keys); w.vec(prefix_key_at); w.i32(position_shift); return w.buf;
   }
   static RequestIn from_bytes(const std::string& s) {
     ByteReader r(s); r.header(TAG_REQUEST_IN); RequestIn q; q.seq_id = r.u64();
     q.prompt_token_ids = r.vec<int32_t>(); q.sampling_params = read_sampling(r);
-    q.affinity_key = r.u64(); q.vision_slots = r.vec<int32_t>(); q.prefix_keys = r.vec<uint64_t>(); q.prefix_key_at = r.vec<int32_t>();
+    q.affinity_key = r.u64(); q.vision_slots = r.vec<int32_t>(); q.prefix_keys = r.vec<uint64_t>(); q.prefix_key_at = r.vec<int32_t>(); q.position_shift = r.i32();
     if (!r.done()) throw WireError("wire: trailing bytes in RequestIn");
     return q;
   }
@@ -152,12 +153,13 @@ struct RequestMigrate {
   int32_t block_size = 64;
   std::vector<uint64_t> prefix_keys;
   std::vector<int32_t> prefix_key_at;
+  int32_t position_shift = 0;
   std::string to_bytes() const {
     ByteWriter w; w.header(TAG_REQUEST_MIGRATE); w.u64(seq_id); w.vec(token_ids); w.i32(prompt_len);
     w.i32(num_computed); write_sampling(w, sampling_params); w.vec(logprobs); w.u64(affinity_key);
     w.vec(migrate_block_table); w.i32(migrate_dp_idx); w.i32(migrate_state_slot); w.i32(migrate_handoff_slot);
     w.i32(migrate_hisparse_slot); w.str(migrate_engine_id); w.i32(migrate_num_kvcache_blocks); w.i32(block_size);
-    w.vec(prefix_keys); w.vec(prefix_key_at);
+    w.vec(prefix_keys); w.vec(prefix_key_at); w.i32(position_shift);
     return w.buf;
   }
   static RequestMigrate from_bytes(const std::string& s) {
@@ -167,7 +169,7 @@ struct RequestMigrate {
     m.migrate_block_table = r.vec<int32_t>(); m.migrate_dp_idx = r.i32(); m.migrate_state_slot = r.i32();
     m.migrate_handoff_slot = r.i32(); m.migrate_hisparse_slot = r.i32(); m.migrate_engine_id = r.str();
     m.migrate_num_kvcache_blocks = r.i32(); m.block_size = r.i32();
-    m.prefix_keys = r.vec<uint64_t>(); m.prefix_key_at = r.vec<int32_t>();
+    m.prefix_keys = r.vec<uint64_t>(); m.prefix_key_at = r.vec<int32_t>(); m.position_shift = r.i32();
     if (!r.done()) throw WireError("wire: trailing bytes in RequestMigrate");
     return m;
   }

@@ -9,6 +9,8 @@ from __future__ import annotations
 import time
 from typing import Dict, Iterable, List, Optional
 
+import numpy as np
+
 from .._native import _core as C
 from ..config import Config
 from ..utils.logging import get_logger
@@ -102,7 +104,12 @@ class LLMEngine:
 
     # ---- requests ----------------------------------------------------------------------------
     def add_request_payload(self, payload: bytes) -> int:
-        return self.scheduler.add_request_bytes(payload)
+        seq_id = self.scheduler.add_request_bytes(payload)
+        shift = self.scheduler.get(seq_id).position_shift
+        if shift:                      # its images stand in the prompt that the prefill engine ran: here its tokens go on behind them
+            self.executor.collective_rpc("register_position_shift", seq_id, shift)
+            self._with_axes.add(seq_id)
+        return seq_id
 
     def add_request(self, prompt_token_ids: List[int], sampling_params=None, seq_id: Optional[int] = None, affinity_key: int = 0) -> int:
         if seq_id is None:
@@ -137,17 +144,17 @@ class LLMEngine:
             raise ValueError("duplicate seq_id")
         slot, ntok = (int(vision_slot.slot), int(vision_slot.num_tokens)) if vision_slot is not None else (-1, 0)
         grids = [list(g) for g in (grid_thw if grid_thw is not None else getattr(vision_slot, "grid_thw", None) or [])]
+        from ..vl.positions import image_positions
         axes = bool(grids) and self.config.model_config.position_axes is not None
-        if axes and self.config.mode != "hybrid":
-            raise ValueError("image positions on several axes stay with the worker that ran the prompt: use mode='hybrid'")
         self.executor.collective_rpc("register_vision", seq_id, list(prompt_token_ids), int(image_token_id), embeddings, pool_desc, slot, ntok,
                                      grids if axes else None, int(spatial_merge_size))
         self._with_axes.add(seq_id)
         self._next_seq_id = max(self._next_seq_id, seq_id) + 1
         sp = sampling_params or C.SamplingParams()
         try:
+            shift = image_positions(np.asarray(prompt_token_ids) == image_token_id, grids, spatial_merge_size)[1] if axes else 0
             at, keys = self.executor.collective_rpc("vision_keys", seq_id)[0] if self.config.enable_prefix_caching else ([], [])
-            return self.scheduler.add_request(C.RequestIn(seq_id, list(prompt_token_ids), sp, 0, [slot] if slot >= 0 else None, keys, at))
+            return self.scheduler.add_request(C.RequestIn(seq_id, list(prompt_token_ids), sp, 0, [slot] if slot >= 0 else None, keys, at, shift))
         except Exception:
             self._release_axes(seq_id)
             raise
@@ -309,6 +316,8 @@ class LLMEngine:
             self.scheduler.complete_migration(ok_ids, True)
         if bad_ids:
             self.scheduler.complete_migration(bad_ids, False)
+            for sid in self._with_axes.intersection(bad_ids):
+                self._release_axes(sid)
 
     # ---- PD ------------------------------------------------------------------------------------
     def export_to_be_migrated(self):

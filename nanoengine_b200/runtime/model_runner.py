@@ -451,6 +451,11 @@ class ModelRunner:
         self.__dict__.setdefault("_vision", {})[int(seq_id)] = [np.concatenate([[0], np.cumsum(is_img)]), is_img, rows, rows.cpu()]
         return embeddings.shape[0]
 
+    def register_position_shift(self, seq_id: int, shift: int) -> None:
+        """A request whose prompt with images another engine has run: its tokens stand `shift` from their index on every axis."""
+        if self.position_axes is not None:
+            self._image_axes[int(seq_id)] = (np.zeros((len(self.position_axes), 1), dtype=np.int64), int(shift))
+
     def vision_keys(self, seq_id: int):
         """(first tokens, keys) of the runs of image tokens of a registered request: a key says in 64 bits what the run stands for, its embeddings as they are
         spliced in and its positions where it has some of its own."""

@@ -150,3 +150,39 @@ def test_preempted_prompts_are_computed_again_with_their_images(axes, kw):
         preempted += sum(v.num_preemptions for v in map(llm.engine.scheduler.get, (1, 2)) if v is not None)
     assert preempted and [out[1], out[2]] == want
     assert not runner._vision and not runner._image_axes and not llm.engine._with_axes
+
+
+@pytest.mark.parametrize("kv", ["float32", "int4"])
+@pytest.mark.parametrize("slot", [True, False])
+def test_prefill_and_decode_engines_place_images_like_one_engine(kv, slot):
+    """The prompt's rows are turned on the prefill engine, what follows goes on behind the images on the decode engine."""
+    from nanoengine_b200.parallel.kv_transfer import KVMigrator, LocalTransport
+    cases = [(1, WIDE), (2, TALL), (3, None)]
+    want = [ask(make(kv), images(i), g)[0] for i, g in cases]
+    prefill, decode = make(kv, mode="prefill", engine_id="p0"), make(kv, mode="decode", engine_id="d0")
+    decode.engine.migrator = KVMigrator(LocalTransport([prefill.engine.executor.runner], [decode.engine.executor.runner]), decode.engine.engine_info(),
+                                        prefill.engine.engine_info())
+    pool = EmbeddingPool(3, 64, 128, "cpu", torch.float32)
+    for i, g in cases:
+        if slot:
+            s = pool.allocate(64)
+            pool.write(s, images(i))
+            kw = dict(vision_slot=VisionSlot("e", s, 64, 128, [list(x) for x in g or []]), pool_desc=pool.export(direct=True))
+        else:
+            kw = dict(embeddings=images(i), grid_thw=g)
+        prefill.engine.add_vision_request(PROMPT, IMG, sampling_params=SP, seq_id=i, **kw)
+    blobs = prefill.generate(return_serialized=True)
+    assert not prefill.engine.executor.runner._vision and not prefill.engine._with_axes
+    first = {}
+    for b in blobs:
+        sid, tok = RequestMigrate.from_bytes(b).metadata
+        first[sid] = tok
+        decode.add_request_payload(b)
+    got = {o["seq_id"]: [first[o["seq_id"]]] + o["token_ids"] for o in decode.generate()}
+    assert [got[i] for i, _ in cases] == want
+    assert not decode.engine.executor.runner._image_axes and not decode.engine._with_axes
+    # a hand-over that fails leaves nothing either
+    decode.engine.migrator.fail_next = True
+    prefill.engine.add_vision_request(PROMPT, IMG, embeddings=images(1), sampling_params=SP, seq_id=9, grid_thw=WIDE)
+    decode.add_request_payload(prefill.generate(return_serialized=True)[-1])
+    assert decode.generate() == [] and not decode.engine.executor.runner._image_axes and not decode.engine._with_axes
