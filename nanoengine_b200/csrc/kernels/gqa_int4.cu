@@ -15,14 +15,17 @@
 // Portions with many rows per key run on the tensor-core prompt kernel over expanded pages instead.
 //
 // A masked nibble is a bf16 pair of subnormals c 2^-133 (16 c 2^-133 for the upper nibble of a byte), so that one fused multiply-add per pair gives
-// (c - 8) s 2^-24, exactly; the 2^24 goes into the softmax scale and the last division.  Scores, maxima, sums and results are 32-bit, probabilities enter
-// the second product as bf16 (2^-9 each) and their sum is a column (row) of ones of the same product.  Every byte stands for a finite value, so a masked key
+// (c - 8) s 2^-24, exactly; the 2^24 goes into the softmax scale and the last division.  Scores, maxima, sums and results are 32-bit.  Probabilities enter
+// the second product as over bf16 pages: heads of 128 without a window as bf16 (2^-8), all others as two bf16 terms (2^-17, a second product on the same unpacked
+// values); their sum is a column (row) of ones of the same products.  One term would be faster where two are taken (us of one / two: 60 x 3000 keys, 16 / 2 heads of
+// 256: 39 / 41, four tokens: 85 / 98; 128 x 4096, 32 / 8 heads of 64: 74 / 83, 64 / 4: 54 / 65; 64 / 4 of 128, window 1000: 34 / 38), but a layer would lose
+// bits with its cache, and its decode steps against its prompts.  Every byte stands for a finite value, so a masked key
 // (probability 0) adds nothing whatever its page holds.
 //
 // Bound by the chain unpack, product, softmax of two (three) warps a scheduler, not by HBM: cycles of a warp for a tile of 64 keys and 16 rows: waiting for copies 290,
 // scores 1460, maximum 290, values 1770, next copy 580; a product and the two pairs that feed it take 9.7 cycles of their pipes, of which none is full (matrix
 // 32 %, integer 31 %, issue slots 41 %).  Measured (B200, calls in a graph, us, GB/s of 6530): 128 x 4096 keys, 64 / 4 heads of 128 (16 rows): 86, 3320;
-// 32 / 8 heads (4 rows): 115, 4960; 2 x 131072 keys, 64 / 4: 50; 60 x 3000, 16 / 2 heads of 256: 40; 33 x 2504, four tokens, 32 / 8: 37; 1 x 1001: 10.  Slower: queries in shared memory, tiles of 32 keys, copies by cp.async, three CTAs per SM with 16 rows (they spill).  tcgen05 with the keys
+// 32 / 8 heads (4 rows): 115, 4960; 2 x 131072 keys, 64 / 4: 50; 60 x 3000, 16 / 2 heads of 256: 41; 33 x 2504, four tokens, 32 / 8: 37; 1 x 1001: 10.  Slower: queries in shared memory, tiles of 32 keys, copies by cp.async, three CTAs per SM with 16 rows (they spill).  tcgen05 with the keys
 // unpacked into tensor memory and the values into shared memory, three CTAs per SM, a warp of its own for copies and products: 116 where this one takes 89; the
 // unpacked values cross shared memory twice, and barriers between unpacking, products and softmax leave the pipes idle.
 #include "kv4.cuh"
@@ -224,7 +227,10 @@ __device__ __forceinline__ I4Scale i4_scale(uint32_t b4) {
 __device__ __forceinline__ uint32_t i4_lower(uint32_t w, const I4Scale& s) { return hfma2_bf16(w & 0x000F000Fu, s.lo, s.z); }
 __device__ __forceinline__ uint32_t i4_upper(uint32_t w, const I4Scale& s) { return hfma2_bf16(w & 0x00F000F0u, s.hi, s.z); }
 
-template <int D, int R, bool kPlain>
+// Two probabilities as bf16, and what that rounding leaves of them, as bf16 again: together 2^-17 of each
+__device__ __forceinline__ uint32_t pair_rest(uint32_t p, float a, float b) { return pack_bf16x2(a - __uint_as_float(p << 16), b - __uint_as_float(p & 0xffff0000u)); }
+
+template <int D, int R, bool kPlain, bool kSplitP>
 __global__ void __launch_bounds__(kI4Threads, I4Geo<D, R>::ctas) gqa_int4_kernel(const I4Args a) {
   using G = I4Geo<D, R>;
   constexpr bool kNarrow = R == 8;                                       // the keys and the value dims are the 16 rows of a product, the query rows its 8 columns
@@ -475,22 +481,30 @@ __global__ void __launch_bounds__(kI4Threads, I4Geo<D, R>::ctas) gqa_int4_kernel
         const float z0 = m0 == -INFINITY ? 0.f : -m0, z1 = m1 == -INFINITY ? 0.f : -m1;
 #pragma unroll
         for (int kk = 0; kk < G::keys / 16; kk++) {
-          uint32_t pr[4];
+          uint32_t pr[4], pl[4];                                         // probabilities; with kSplitP what their rounding leaves
           if constexpr (kNarrow) {
             // a lane has two rows of one key, the product wants two keys of one row
 #pragma unroll
-            for (int t = 0; t < 2; t++)
-              pr[t] = transpose_8x8(pack_bf16x2(exp2f(fmaf(s[kk][2 * t], scale, z0)), exp2f(fmaf(s[kk][2 * t + 1], scale, z1))));
+            for (int t = 0; t < 2; t++) {
+              const float x = exp2f(fmaf(s[kk][2 * t], scale, z0)), y = exp2f(fmaf(s[kk][2 * t + 1], scale, z1));
+              const uint32_t p2 = pack_bf16x2(x, y);
+              pr[t] = transpose_8x8(p2);
+              if constexpr (kSplitP) pl[t] = transpose_8x8(pair_rest(p2, x, y));
+            }
             const uint32_t ones[4] = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
             mma_16816(l, ones, pr[0], pr[1]);                            // the sum of the probabilities as they are rounded
+            if constexpr (kSplitP) mma_16816(l, ones, pl[0], pl[1]);
           } else {
 #pragma unroll
           for (int t = 0; t < 2; t++) {
             const float (&v)[4] = s[2 * kk + t];
-            pr[2 * t] = pack_bf16x2(exp2f(fmaf(v[0], scale, z0)), exp2f(fmaf(v[1], scale, z0)));
-            pr[2 * t + 1] = pack_bf16x2(exp2f(fmaf(v[2], scale, z1)), exp2f(fmaf(v[3], scale, z1)));
+            const float x0 = exp2f(fmaf(v[0], scale, z0)), x1 = exp2f(fmaf(v[1], scale, z0)), y0 = exp2f(fmaf(v[2], scale, z1)), y1 = exp2f(fmaf(v[3], scale, z1));
+            pr[2 * t] = pack_bf16x2(x0, x1);
+            pr[2 * t + 1] = pack_bf16x2(y0, y1);
+            if constexpr (kSplitP) { pl[2 * t] = pair_rest(pr[2 * t], x0, x1); pl[2 * t + 1] = pair_rest(pr[2 * t + 1], y0, y1); }
           }
           mma_16816(l, pr, 0x3F803F80u, 0x3F803F80u);
+          if constexpr (kSplitP) mma_16816(l, pl, 0x3F803F80u, 0x3F803F80u);
           }
           // values: this lane's four keys of the step, an eighth of each row
           uint32_t w[4][G::vwords], sb[4];
@@ -510,8 +524,15 @@ __global__ void __launch_bounds__(kI4Threads, I4Geo<D, R>::ctas) gqa_int4_kernel
             const uint32_t al = __byte_perm(w[0][i], w[1][i], 0x5410), ah = __byte_perm(w[0][i], w[1][i], 0x7632);
             const uint32_t bl = __byte_perm(w[2][i], w[3][i], 0x5410), bh = __byte_perm(w[2][i], w[3][i], 0x7632);
             auto both = [&](int j, uint32_t a0, uint32_t b0, uint32_t a1, uint32_t b1) {       // dims j and j + 1 of the lane's eight: first keys, second keys
-              if constexpr (kNarrow) { const uint32_t x[4] = {a0, a1, b0, b1}; mma_16816(o[4 * i + j / 2], x, pr[0], pr[1]); }
-              else { mma_16816(o[kNarrow ? 0 : 8 * i + j], pr, a0, b0); mma_16816(o[kNarrow ? 0 : 8 * i + j + 1], pr, a1, b1); }
+              if constexpr (kNarrow) {
+                const uint32_t x[4] = {a0, a1, b0, b1};
+                mma_16816(o[4 * i + j / 2], x, pr[0], pr[1]);
+                if constexpr (kSplitP) mma_16816(o[4 * i + j / 2], x, pl[0], pl[1]);
+              } else {
+                mma_16816(o[kNarrow ? 0 : 8 * i + j], pr, a0, b0);
+                mma_16816(o[kNarrow ? 0 : 8 * i + j + 1], pr, a1, b1);
+                if constexpr (kSplitP) { mma_16816(o[kNarrow ? 0 : 8 * i + j], pl, a0, b0); mma_16816(o[kNarrow ? 0 : 8 * i + j + 1], pl, a1, b1); }
+              }
             };
             both(0, i4_lower(al, sa), i4_lower(bl, sz), i4_lower(ah, sa), i4_lower(bh, sz));
             both(2, i4_upper(al, sa), i4_upper(bl, sz), i4_upper(ah, sa), i4_upper(bh, sz));
@@ -645,20 +666,24 @@ __global__ void __launch_bounds__(i4_join_threads(kSplit)) gqa_int4_join_kernel(
 using namespace ne;
 
 namespace {
-template <int D, int R, bool kPlain> cudaError_t launch_i4_main(const I4Args& a, cudaStream_t st) {
+template <int D, int R, bool kPlain, bool kSplitP> cudaError_t launch_i4_main(const I4Args& a, cudaStream_t st) {
   static bool configured[64] = {};                                       // per device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !configured[dev]) {
-    e = cudaFuncSetAttribute(gqa_int4_kernel<D, R, kPlain>, cudaFuncAttributeMaxDynamicSharedMemorySize, I4Geo<D, R>::smem);
+    e = cudaFuncSetAttribute(gqa_int4_kernel<D, R, kPlain, kSplitP>, cudaFuncAttributeMaxDynamicSharedMemorySize, I4Geo<D, R>::smem);
     if (e != cudaSuccess) return e;
     if (dev < 64) configured[dev] = true;
   }
-  return launch_pdl(gqa_int4_kernel<D, R, kPlain>, dim3((unsigned)(a.shares / kI4Warps)), dim3(kI4Threads), I4Geo<D, R>::smem, st, a);
+  return launch_pdl(gqa_int4_kernel<D, R, kPlain, kSplitP>, dim3((unsigned)(a.shares / kI4Warps)), dim3(kI4Threads), I4Geo<D, R>::smem, st, a);
+}
+template <int D, int R, bool kSplitP> cudaError_t launch_i4_pages(const I4Args& a, cudaStream_t st) {
+  return a.block_size % I4Geo<D, R>::keys == 0 ? launch_i4_main<D, R, true, kSplitP>(a, st) : launch_i4_main<D, R, false, kSplitP>(a, st);
 }
 template <int D, int R> cudaError_t launch_i4_rows(const I4Args& a, cudaStream_t st) {
-  return a.block_size % I4Geo<D, R>::keys == 0 ? launch_i4_main<D, R, true>(a, st) : launch_i4_main<D, R, false>(a, st);
+  if constexpr (D == 128) { if (a.window <= 0) return launch_i4_pages<D, R, false>(a, st); }
+  return launch_i4_pages<D, R, true>(a, st);
 }
 template <int D> int launch_i4(const I4Args& a, int tiles, cudaStream_t st) {
   const cudaError_t e = a.rows == 8 ? launch_i4_rows<D, 8>(a, st) : launch_i4_rows<D, 16>(a, st);

@@ -229,7 +229,7 @@ def _rows16(t):
 
 
 def gqa_attention_paged(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale, window: int = 0):
-    """`window` > 0: every query sees only its last `window` key positions (sliding-window layers).  bf16 caches of 64-token pages: tensor cores.  Those
+    """`window` > 0: every query sees only its last `window` key positions (sliding-window layers).  bf16 caches of 64-token pages, and 4-bit ones: tensor cores.  Those
     layers, and head sizes other than 128, keep their probabilities in 32-bit (two bf16 terms); other caches run on the generic kernel."""
     if k_cache.dtype == torch.uint8:
         return _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale, window)
@@ -300,8 +300,8 @@ def _int4_expanded_bytes(B: int, W: int, Hkv: int, D: int, bs: int) -> int:
 def _int4_min_rows(Hq: int, Hkv: int, D: int) -> int:
     """Rows (tokens times heads of a group) a sequence, in the mean, from which a step runs over pages expanded to bf16; 0: never.
     Unpacking for every 16 rows then costs more than expanding the context once.  us of the kernel / of expanding, then the prompt kernel: 32 x 4096 keys, 64 / 4 heads of 128:
-    64 rows 89 / 157, 128: 161 / 157, 256: 301 / 168; 16 / 2 heads of 256: 64: 110 / 185, 128: 192 / 185; 16 x 4096, 16 / 2 heads of 64: 256: 57 / 83, 512: 98 / 90;
-    4 x 4096, 64 / 4 of 128: 128: 34 / 57, 512: 87 / 74."""
+    64 rows 86 / 149, 128: 160 / 153; 16 / 2 heads of 256: 64: 122 / 184, 128: 219 / 181; 16 x 4096, 16 / 2 heads of 64: 256: 65 / 77, 512: 117 / 86;
+    4 x 4096, 64 / 4 of 128: 128: 32 / 37, 512: 85 / 72."""
     g = Hq // Hkv
     return (512 if D == 64 else 128) if (g % 4 == 0 or g == 1 and Hq % 4 == 0) and g <= 128 else 0
 
@@ -315,7 +315,8 @@ def int4_expansion_room(max_tokens: int, max_seqs: int, max_len: int, Hq: int, H
 
 
 def _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale, window: int):
-    """4-bit pages: a kernel that unpacks them in registers for steps of few query rows per key, the tensor-core kernels over pages expanded to bf16 for others."""
+    """4-bit pages: a kernel that unpacks them in registers for steps of few query rows per key, the tensor-core kernels over pages expanded to bf16 for others; both
+    keep the probabilities as `gqa_attention_paged` says."""
     T, Hq, D = q.shape
     Hkv = k_cache.shape[1] if k_cache.dim() > 1 else 0
     bs = _k._kv4_dims(k_cache, v_cache, Hkv, D)
@@ -340,8 +341,8 @@ def _gqa_int4(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, sca
     if many and T * g >= many * B and _int4_expanded_bytes(B, W, Hkv, D, bs) <= _INT4_EXPANDED_BYTES:
         k, v, bt, cl = _k.kv4_expand(k_cache, v_cache, bt, cl, D)
         return _gqa_pages(q, k, v, bt, cu, cl, scale, window, own_pages=True)
-    # Row tiles of 8 where a sequence has no more rows of a kv head, else of 16.  us of 16 / 8: 128 x 4096 keys, 32 / 8 heads of 128: 159 / 116, of 64: 96 / 75;
-    # 60 x 3000, 16 / 2 heads of 256: 53 / 41.
+    # Row tiles of 8 where a sequence has no more rows of a kv head, else of 16.  us of 16 / 8: 128 x 4096 keys, 32 / 8 heads of 128: 155 / 115, of 64: 115 / 83;
+    # 60 x 3000, 16 / 2 heads of 256: 57 / 41.
     rows = 8 if T * g <= 8 * B else 16
     # equal shares of the batch's work, one for every warp that is resident at once, but no more than its tiles of keys need
     per_sm = _INT4_SHARES.get((D, rows))

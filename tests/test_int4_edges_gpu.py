@@ -232,3 +232,30 @@ def test_the_room_of_expanded_pages_stays_outside_the_cache(kv, monkeypatch):
     sp = SamplingParams(temperature=0.0, max_tokens=1, ignore_eos=True)
     llm.generate([[5 + i % 400 for i in range(3900)]], sp)
     assert kv == "auto" or seen[0] >= 4 * 3904 * 2 * 128
+
+
+KEPT = [
+    # hq, hkv, dim, block size, new, contexts, window: row tiles of 8 and of 16, tiles that lie in a page and that do not, contexts cut into pieces and not
+    (16, 2, 256, 64, [1] * 5, [300, 1, 64, 65, 2000], 0),
+    (16, 2, 256, 16, [4, 3], [90, 700], 0),
+    (64, 4, 256, 64, [1, 2], [40, 5000], 0),
+    (16, 4, 64, 64, [1, 1], [129, 3000], 0),
+    (32, 2, 64, 32, [1, 3], [77, 1500], 0),
+    (32, 8, 128, 64, [1, 1], [900, 64], 100),
+    (64, 4, 128, 16, [1, 2], [900, 333], 70),
+    (16, 2, 256, 64, [2], [3001], 1000),
+]
+
+
+@pytest.mark.parametrize("hq,hkv,dim,bs,new,ctx,window", KEPT)
+def test_probabilities_of_windows_and_of_heads_that_are_not_128_wide_keep_17_bits(hq, hkv, dim, bs, new, ctx, window):
+    """As over bf16 pages.  Weights w_i (1 + d_i), |d_i| <= e = 2^-17 (a probability as bf16, off by at most 2^-8 of its power of two, and the rest as bf16 again, normalised by
+    their own sum, are off by e (1 + 2 e) sum w |v - o|; the result is rounded once; 32-bit scores and exponentials as in `attention_bound`."""
+    from nanoengine_b200.ops import sm100_attn
+    args, out, _ = case(hq, hkv, dim, bs, new, ctx, window, seed=12)
+    _, spread, mass, top = dense_attention(args[0], cache_values(args[1], dim), cache_values(args[2], dim), args[3].cpu(), new, ctx, args[6], window)
+    e = 2.0 ** -17
+    before = sm100_attn.INT4_CALLS[0]
+    got = ops.gqa_attention_paged(*args)
+    assert sm100_attn.INT4_CALLS[0] == before + 1
+    within(got, out, BF16_HALF_STEP * out.abs() + (1 + BF16_HALF_STEP) * (e * (1 + 2 * e) * spread + (2.0 ** -15 * top + 2.0 ** -18) * mass) + 1e-30)
