@@ -12,8 +12,11 @@
 // an element or a scale lies nearer to a border than that (one step of two rows in a hundred), its warp computes it again in 64.  Value rows are bf16,
 // whose quotients are exact or far from a border in 32 bits.  Built without approximate functions.
 //
-// Measured (B200, us, calls in a graph; bytes at 6530 GB/s): 64 / 4 heads of 128 into 4 bits, three axes: 128 tokens 4.4, 4096: 37 (22); 32 / 8 heads into bf16, three axes: 4096: 23 (15);
-// bound there by the chain position, table row, rotation of few resident warps.  4096 rows read back (8 heads): 5.8.  Expanding 32 x 4096 keys of 4 heads: 79 (52).
+// Measured (B200, us, calls in a graph over inputs larger than L2; bytes at 6540 GB/s): 64 / 4 heads of 128 into 4 bits, three axes: 128 tokens 5.0, 4096: 39 (22), one
+// position: 34; 16 / 2 of 256: 26 (12); 32 / 8 heads into bf16, three axes: 4096: 24 (15); bound there by the chain position, table row, rotation of few resident warps: eight CTAs
+// per SM cap them at 64 registers, where the 4-bit forms spill 172 to 184 bytes (the 64-bit pass of key rows), the bf16 ones 16 to 44.  Rows stored as they are: 4096
+// of 8 heads of 128: 19 (3.2), of 2 heads of 256: 10 (1.6); read back: 6.5 and 3.9.  Expanding 32 x 4096 keys of 4 heads: 79 (52): a page's rows are found behind a barrier,
+// codes come as 4 bytes and scales as single ones.
 #include "kv4.cuh"
 
 namespace ne {
