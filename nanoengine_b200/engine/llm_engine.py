@@ -105,7 +105,8 @@ class LLMEngine:
     # ---- requests ----------------------------------------------------------------------------
     def add_request_payload(self, payload: bytes) -> int:
         seq_id = self.scheduler.add_request_bytes(payload)
-        shift = self.scheduler.get(seq_id).position_shift
+        seq = self.scheduler.get(seq_id)
+        shift = seq.position_shift if seq.num_computed else 0
         if shift:                      # its images stand in the prompt that the prefill engine ran: here its tokens go on behind them
             self.executor.collective_rpc("register_position_shift", seq_id, shift)
             self._with_axes.add(seq_id)
@@ -140,6 +141,8 @@ class LLMEngine:
         pages of image tokens, and those behind them, between prompts of the same images at the same places only.  Parity: reference engine/llm_component.py:285-340 + runtime/runner/model_runner.py:1557-1573, :1886-1890."""
         if seq_id is None:
             seq_id = self._next_seq_id
+        if self.config.pp > 1:                               # stages pass hidden rows on, none of them splices images in
+            raise ValueError("prompts with images run without pipeline stages (pp = 1)")
         if self.scheduler.get(seq_id) is not None:           # before its images take the place of a live request's
             raise ValueError("duplicate seq_id")
         slot, ntok = (int(vision_slot.slot), int(vision_slot.num_tokens)) if vision_slot is not None else (-1, 0)

@@ -186,3 +186,19 @@ def test_prefill_and_decode_engines_place_images_like_one_engine(kv, slot):
     prefill.engine.add_vision_request(PROMPT, IMG, embeddings=images(1), sampling_params=SP, seq_id=9, grid_thw=WIDE)
     decode.add_request_payload(prefill.generate(return_serialized=True)[-1])
     assert decode.generate() == [] and not decode.engine.executor.runner._image_axes and not decode.engine._with_axes
+
+
+def test_images_under_pipeline_stages_are_refused(monkeypatch):
+    llm = make(mode="prefill")
+    monkeypatch.setattr(llm.engine.config, "pp", 2)
+    with pytest.raises(ValueError, match="pipeline"):
+        llm.engine.add_vision_request(PROMPT, IMG, embeddings=images(1), sampling_params=SP, grid_thw=WIDE)
+    assert not llm.engine._with_axes and llm.engine.scheduler.num_waiting() == 0
+
+
+def test_a_prompt_that_no_engine_has_run_stands_at_its_index():
+    """Only a hand-over says how far tokens stand from their index; a prompt of its own is placed by its images."""
+    want = make().generate([PROMPT], SP)[0]["token_ids"]
+    llm = make()
+    llm.engine.add_request_payload(C.RequestIn(1, PROMPT, SP, position_shift=9).to_bytes())
+    assert not llm.engine._with_axes and llm.generate()[0]["token_ids"] == want
