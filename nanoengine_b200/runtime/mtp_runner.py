@@ -129,7 +129,8 @@ class MTPRunner:
     def _run_prefill(self, b, ctx: ForwardContext):
         r = self.r
         ids, pos = ctx.extras["input_ids"], ctx.extras["positions"]
-        hidden = r.model(ids, pos, ctx)
+        embeds = ctx.extras.get("inputs_embeds")
+        hidden = r.model(ids, pos, ctx) if embeds is None else r.model(ids, pos, ctx, inputs_embeds=embeds)
         mask = np.asarray(b.sample_mask, dtype=bool)
         temps = torch.tensor(list(b.temperatures), dtype=torch.float32, device=r.device)
         rows = ctx.last_token_indices.long()

@@ -202,3 +202,19 @@ def test_a_prompt_that_no_engine_has_run_stands_at_its_index():
     llm = make()
     llm.engine.add_request_payload(C.RequestIn(1, PROMPT, SP, position_shift=9).to_bytes())
     assert not llm.engine._with_axes and llm.generate()[0]["token_ids"] == want
+
+
+def test_images_with_speculative_decoding():
+    """Prompts of an engine that drafts splice the image rows in like those of others."""
+    from nanoengine_b200.models.config import tiny_deepseek_v3
+    got = []
+    for spec in (0, 2):
+        mc = tiny_deepseek_v3()
+        mc.num_nextn_predict_layers = 1
+        llm = LLM(Config(model="tiny-deepseek-v3", model_config=mc, dummy_weight=True, dtype="float32", device="cpu", kvcache_block_size=16, num_kvcache_blocks=32,
+                         max_num_seqs=4, num_speculative_tokens=spec, seed=0))
+        for seed in (1, 2):
+            emb = torch.randn(6, mc.hidden_size, generator=torch.Generator().manual_seed(seed)) * 0.5
+            llm.engine.add_vision_request([3, 11] + [IMG] * 6 + list(range(30, 60)), IMG, embeddings=emb, sampling_params=SP, seq_id=seed)
+        got.append([o["token_ids"] for o in sorted(llm.generate(), key=lambda o: o["seq_id"])])
+    assert got[0] == got[1] and got[0][0] != got[0][1]
